@@ -52,13 +52,21 @@ EXPORTED_SYMBOLS = (
     "fh_xent_fwd",
     "fh_xent_bwd",
     "fh_xent_bwd_bwd",
+    "fh_embed_scratch_bytes",
+    "fh_embed_fwd",
+    "fh_embed_bwd",
+    "fh_embed_bwd_bwd",
+    "fh_dropout",
+    "fh_policy_fwd",
+    "fh_policy_bwd",
+    "fh_policy_bwd_bwd",
     "fh_device_status",
     "fh_status_string",
     "fh_last_error",
     "fh_abi_version",
     "fh_launch_count",
 )
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 
 class FlashHogError(RuntimeError):
@@ -127,6 +135,15 @@ def lib() -> ctypes.CDLL:
     h.fh_xent_fwd.argtypes = [vp, i32, i32, i32, ll, vp, vp, vp, vp]
     h.fh_xent_bwd.argtypes = [vp, i32, i32, i32, ll, vp, vp, vp, vp, f32, vp]
     h.fh_xent_bwd_bwd.argtypes = [vp, i32, i32, i32, ll, vp, vp, vp, vp, f32, vp, vp, vp]
+    h.fh_embed_scratch_bytes.argtypes = [i32, i32]
+    h.fh_embed_scratch_bytes.restype = ll
+    h.fh_embed_fwd.argtypes = [vp, i32, i32, i32, i32, vp, vp, f32, vp]
+    h.fh_embed_bwd.argtypes = [vp, i32, i32, i32, i32, vp, vp, f32, ll, vp, vp]
+    h.fh_embed_bwd_bwd.argtypes = [vp, i32, i32, i32, i32, vp, vp, f32, ll, vp]
+    h.fh_dropout.argtypes = [vp, ll, i32, vp, i32, vp, i32, vp, vp, ctypes.c_uint, i32]
+    h.fh_policy_fwd.argtypes = [vp, i32, i32, i32, ll] + [vp] * 6 + [f32] * 4 + [vp] * 3
+    h.fh_policy_bwd.argtypes = [vp, i32, i32, i32, ll] + [vp] * 5
+    h.fh_policy_bwd_bwd.argtypes = [vp, i32, i32, i32, ll] + [vp] * 7
     h.fh_device_status.argtypes = [vp, ctypes.POINTER(ctypes.c_int)]
     h.fh_status_string.argtypes = [i32]
     h.fh_status_string.restype = ctypes.c_char_p
@@ -139,7 +156,8 @@ def lib() -> ctypes.CDLL:
                  "fh_attn_bwdbwd_o", "fh_attn_bwdbwd_noalloc", "fh_attn_jvp_bwd", "fh_attn_fwd_f32",
                  "fh_attn_bwd_f32", "fh_attn_bwdbwd_f32", "fh_attn_jvp_bwd_f32", "fh_device_status",
                  "fh_abi_version", "fh_layernorm_fwd", "fh_layernorm_bwd", "fh_layernorm_bwd_bwd", "fh_gelu",
-                 "fh_xent_fwd", "fh_xent_bwd", "fh_xent_bwd_bwd"):
+                 "fh_xent_fwd", "fh_xent_bwd", "fh_xent_bwd_bwd", "fh_embed_fwd", "fh_embed_bwd", "fh_embed_bwd_bwd",
+                 "fh_dropout", "fh_policy_fwd", "fh_policy_bwd", "fh_policy_bwd_bwd"):
         getattr(h, name).restype = i32
     if h.fh_abi_version() != ABI_VERSION:
         raise RuntimeError(f"flash_hog_b200 ABI mismatch: library {h.fh_abi_version()}, binding {ABI_VERSION}")
@@ -159,6 +177,28 @@ def _ptr(t):
 
 def _stream(device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _on_device(f):
+    """Runs a wrapper with its first argument's device current: on a default stream the
+    library launches on the current device."""
+
+    @functools.wraps(f)
+    def call(t, *args, **kwargs):
+        if not t.is_cuda or t.device.index == torch.cuda.current_device():
+            return f(t, *args, **kwargs)
+        with torch.cuda.device(t.device):
+            return f(t, *args, **kwargs)
+
+    return call
+
+
+def _same_device(t: torch.Tensor, *others) -> None:
+    if not t.is_cuda:
+        raise ValueError("flash_hog_b200 runs on CUDA tensors only")
+    for x in others:
+        if x is not None and x.device != t.device:
+            raise ValueError(f"tensors must be on one CUDA device, got {t.device} and {x.device}")
 
 
 def _strides(t: torch.Tensor) -> FhStrides:
@@ -432,6 +472,106 @@ def xent_bwd_bwd(z, t, lse, g, s: float, u, gz, gg) -> None:
             raise ValueError("u and gz are contiguous tensors of the logits' shape and dtype")
     _check("fh_xent_bwd_bwd", lib().fh_xent_bwd_bwd(_stream(z.device), dt, rows, vocab, ld, _ptr(z), _ptr(t),
                                                      _ptr(lse), _ptr(g), float(s), _ptr(u), _ptr(gz), _ptr(gg)))
+
+
+def _embed_args(rows, table, tokens):
+    """(dtype, n, vocab, dim) of (n, dim) rows against a (vocab, dim) table."""
+    _same_device(table, rows, tokens)
+    if table.dim() != 2 or table.dtype not in _GELU_DTYPES or not table.is_contiguous():
+        raise ValueError("an embedding table is a contiguous (vocab, dim) fp32 or bf16 tensor")
+    if tokens.dtype != torch.int64 or not tokens.is_contiguous():
+        raise ValueError("embedding tokens are a contiguous int64 tensor")
+    n, (vocab, dim) = tokens.numel(), table.shape
+    if rows.dtype != table.dtype or not rows.is_contiguous() or rows.numel() != n * dim:
+        raise ValueError("embedding rows are a contiguous (tokens, dim) tensor of the table's dtype")
+    if n >= 2 ** 31 or vocab >= 2 ** 31 - 1:
+        raise ValueError("embedding: fewer than 2^31 tokens and 2^31 - 1 table rows")
+    return _GELU_DTYPES[table.dtype], n, vocab, dim
+
+
+@_on_device
+def embed_fwd(w, tokens, scale: float, y) -> None:
+    """y_i = scale w[t_i]; see fh_embed_fwd."""
+    args = _embed_args(y, w, tokens)
+    _check("fh_embed_fwd", lib().fh_embed_fwd(_stream(w.device), *args, _ptr(w), _ptr(tokens), float(scale), _ptr(y)))
+
+
+@_on_device
+def embed_bwd(dy, tokens, scale: float, padding_idx: int, dw) -> None:
+    """dw[v] = scale sum_{t_i = v} dy_i; see fh_embed_bwd."""
+    args = _embed_args(dy, dw, tokens)
+    scratch = torch.empty(int(lib().fh_embed_scratch_bytes(args[1], args[3])), dtype=torch.uint8, device=dw.device)
+    _check("fh_embed_bwd", lib().fh_embed_bwd(_stream(dw.device), *args, _ptr(dy), _ptr(tokens), float(scale),
+                                             int(padding_idx), _ptr(dw), _ptr(scratch)))
+
+
+@_on_device
+def embed_bwd_bwd(ddw, tokens, scale: float, padding_idx: int, ddy) -> None:
+    """ddy_i = scale ddw[t_i], 0 for padding; see fh_embed_bwd_bwd."""
+    args = _embed_args(ddy, ddw, tokens)
+    _check("fh_embed_bwd_bwd", lib().fh_embed_bwd_bwd(_stream(ddw.device), *args, _ptr(ddw), _ptr(tokens),
+                                                     float(scale), int(padding_idx), _ptr(ddy)))
+
+
+@_on_device
+def dropout(x, res, y, seed, subsequence: int, limit: int) -> None:
+    """y = res + keep x / (1 - limit / 65536); see fh_dropout. ``res`` may be None."""
+    _same_device(x, res, y, seed)
+    if seed.dtype != torch.int64 or seed.numel() != 1:
+        raise ValueError("the dropout seed is an int64 tensor of one element")
+    for t in (x, res, y):
+        if t is not None and (t.dtype not in _GELU_DTYPES or not t.is_contiguous() or t.shape != x.shape):
+            raise ValueError("dropout tensors are contiguous fp32 or bf16 tensors of one shape")
+    _check("fh_dropout", lib().fh_dropout(
+        _stream(x.device), x.numel(), _GELU_DTYPES[x.dtype], _ptr(x), 0 if res is None else _GELU_DTYPES[res.dtype],
+        _ptr(res), _GELU_DTYPES[y.dtype], _ptr(y), _ptr(seed), int(subsequence), int(limit)))
+
+
+def _policy_args(z, actions, *vectors):
+    """(dtype, rows, vocab, ld) of the logits; ``vectors``: fp32 tensors of one entry per row, or None."""
+    _same_device(z, actions, *vectors)
+    if z.dim() != 2 or z.dtype not in _GELU_DTYPES or z.shape[1] < 1 or (z.stride(1) != 1 and z.shape[1] > 1):
+        raise ValueError("policy logits are a (rows, vocab) fp32 or bf16 tensor with unit column stride")
+    rows, vocab = z.shape
+    if actions.dtype != torch.int64 or not actions.is_contiguous() or actions.shape != (rows,):
+        raise ValueError("policy actions are a contiguous int64 vector of one entry per row")
+    for v in vectors:
+        if v is not None and (v.dtype != torch.float32 or not v.is_contiguous() or v.shape != (rows,)):
+            raise ValueError("the policy's per-row inputs are contiguous fp32 vectors of one entry per row")
+    return _GELU_DTYPES[z.dtype], rows, vocab, z.stride(0) if rows > 1 else vocab
+
+
+@_on_device
+def policy_fwd(z, actions, old, adv, ref, weights, clip_low: float, clip_high: float, kl_coef: float,
+               normalizer: float, lp, loss, stats) -> None:
+    """Loss, log probabilities and the backward's statistics; see fh_policy_fwd."""
+    args = _policy_args(z, actions, old, adv, ref, weights, lp)
+    _check("fh_policy_fwd", lib().fh_policy_fwd(
+        _stream(z.device), *args, _ptr(z), _ptr(actions), _ptr(old), _ptr(adv), _ptr(ref), _ptr(weights),
+        float(clip_low), float(clip_high), float(kl_coef), float(normalizer), _ptr(lp), _ptr(loss), _ptr(stats)))
+
+
+@_on_device
+def policy_bwd(z, actions, stats, g, dz) -> None:
+    """dz = g dloss/dz; g a one-element fp32 device tensor."""
+    args = _policy_args(z, actions)
+    _same_device(z, stats, g, dz)
+    if dz.dtype != z.dtype or not dz.is_contiguous() or dz.shape != z.shape:
+        raise ValueError("dz is a contiguous tensor of the logits' shape and dtype")
+    _check("fh_policy_bwd", lib().fh_policy_bwd(_stream(z.device), *args, _ptr(z), _ptr(actions), _ptr(stats),
+                                               _ptr(g), _ptr(dz)))
+
+
+@_on_device
+def policy_bwd_bwd(z, actions, stats, g, u, gz, gg) -> None:
+    """Backward's backward given the cotangent u of dz; see fh_policy_bwd_bwd."""
+    args = _policy_args(z, actions, gg)
+    _same_device(z, stats, g, u, gz)
+    for x in (u, gz):
+        if x.dtype != z.dtype or not x.is_contiguous() or x.shape != z.shape:
+            raise ValueError("u and gz are contiguous tensors of the logits' shape and dtype")
+    _check("fh_policy_bwd_bwd", lib().fh_policy_bwd_bwd(_stream(z.device), *args, _ptr(z), _ptr(actions), _ptr(stats),
+                                                       _ptr(g), _ptr(u), _ptr(gz), _ptr(gg)))
 
 
 def launch_count() -> int:

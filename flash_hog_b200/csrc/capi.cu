@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -553,6 +554,136 @@ int fh_xent_bwd_bwd(void* stream, int dtype, int rows, int vocab, long long ld, 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if ((rc = select_stream_device(st)) != kOk) return rc;
   return launch_xent(2, dtype == 1, rows, vocab, ld, z, t, const_cast<float*>(lse), nullptr, g, s, u, gz, gg, st);
+}
+
+// ------------------------------------------------------------------------------------
+// Embedding, dropout and the clipped policy loss
+// ------------------------------------------------------------------------------------
+
+static int embed_check(int dtype, int n, int vocab, int dim, const void* x, const long long* tokens, const void* y) {
+  g_last_error[0] = 0;
+  if (n < 0 || vocab < 1 || vocab == 0x7fffffff || dim < 1 || dim > (1 << 20) || (dtype != 0 && dtype != 1))
+    return fail(FH_ERR_INVALID_ARGUMENT,
+                "embed: n >= 0, vocab in [1, 2^31 - 2], dim in [1, 2^20], dtype 0 (fp32) or 1 (bf16)");
+  if (n > 0 && (!x || !tokens || !y)) return fail(FH_ERR_INVALID_ARGUMENT, "embed: a tensor pointer is NULL");
+  return kOk;
+}
+
+long long fh_embed_scratch_bytes(int n, int dim) {
+  if (embed_check(0, n, 1, dim, &n, reinterpret_cast<const long long*>(&n), &n) != kOk) return -1;
+  return embed_scratch_bytes(n, dim);
+}
+
+int fh_embed_fwd(void* stream, int dtype, int n, int vocab, int dim, const void* w, const long long* tokens,
+                 float scale, void* y) {
+  if (injected("fh_embed_fwd")) return FH_ERR_INJECTED;
+  int rc = embed_check(dtype, n, vocab, dim, w, tokens, y);
+  if (rc != kOk || n == 0) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = select_stream_device(st)) != kOk) return rc;
+  return launch_embed_lookup(dtype == 1, n, vocab, dim, tokens, w, scale, -1, NAN, y, st);
+}
+
+int fh_embed_bwd(void* stream, int dtype, int n, int vocab, int dim, const void* dy, const long long* tokens,
+                 float scale, long long padding_idx, void* dw, void* scratch) {
+  if (injected("fh_embed_bwd")) return FH_ERR_INJECTED;
+  int rc = embed_check(dtype, n, vocab, dim, dy, tokens, dw);
+  if (rc != kOk) return rc;
+  if (!all_aligned(dw) || (n > 0 && !all_aligned(scratch)))
+    return fail(FH_ERR_INVALID_ARGUMENT, "embed: dw and scratch must be 16-byte aligned");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = select_stream_device(st)) != kOk) return rc;
+  return launch_embed_grad(dtype == 1, n, vocab, dim, tokens, dy, scale, padding_idx, dw, scratch, st);
+}
+
+int fh_embed_bwd_bwd(void* stream, int dtype, int n, int vocab, int dim, const void* ddw, const long long* tokens,
+                     float scale, long long padding_idx, void* ddy) {
+  if (injected("fh_embed_bwd_bwd")) return FH_ERR_INJECTED;
+  int rc = embed_check(dtype, n, vocab, dim, ddw, tokens, ddy);
+  if (rc != kOk || n == 0) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = select_stream_device(st)) != kOk) return rc;
+  return launch_embed_lookup(dtype == 1, n, vocab, dim, tokens, ddw, scale, padding_idx, 0.f, ddy, st);
+}
+
+int fh_dropout(void* stream, long long n, int x_dtype, const void* x, int res_dtype, const void* res, int y_dtype,
+               void* y, const long long* seed, unsigned int subsequence, int limit) {
+  if (injected("fh_dropout")) return FH_ERR_INJECTED;
+  g_last_error[0] = 0;
+  auto dtype_ok = [](int d) { return d == 0 || d == 1; };
+  if (n < 0 || !dtype_ok(x_dtype) || !dtype_ok(y_dtype) || (res && !dtype_ok(res_dtype)) || limit < 0 || limit > 65536)
+    return fail(FH_ERR_INVALID_ARGUMENT, "dropout: n >= 0, dtypes 0 (fp32) or 1 (bf16), limit in [0, 65536]");
+  if (res && y_dtype != (x_dtype & res_dtype))
+    return fail(FH_ERR_INVALID_ARGUMENT, "dropout: with a residual y is bf16 where both inputs are, else fp32");
+  if (n == 0) return FH_OK;
+  if (!x || !y || !seed) return fail(FH_ERR_INVALID_ARGUMENT, "dropout: x, y and seed are required");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int rc = select_stream_device(st);
+  if (rc != kOk) return rc;
+  const float factor = limit < 65536 ? 65536.f / static_cast<float>(65536 - limit) : 0.f;
+  return launch_dropout(x_dtype == 1, res && res_dtype == 1, y_dtype == 1, n, x, res, y, seed, subsequence,
+                        static_cast<unsigned>(limit), factor, st);
+}
+
+static int policy_check(int dtype, int rows, int vocab, long long ld, const void* z, const long long* actions,
+                        const float* stats) {
+  g_last_error[0] = 0;
+  if (rows < 0 || vocab < 1 || ld < vocab || (dtype != 0 && dtype != 1))
+    return fail(FH_ERR_INVALID_ARGUMENT, "policy: rows >= 0, vocab >= 1, ld >= vocab, dtype 0 (fp32) or 1 (bf16)");
+  if (!stats || (rows > 0 && (!z || !actions)))
+    return fail(FH_ERR_INVALID_ARGUMENT, "policy: logits, actions and stats are required");
+  return kOk;
+}
+
+int fh_policy_fwd(void* stream, int dtype, int rows, int vocab, long long ld, const void* z, const long long* actions,
+                  const float* old, const float* adv, const float* ref, const float* weights, float clip_low,
+                  float clip_high, float kl_coef, float normalizer, float* lp, float* loss, float* stats) {
+  if (injected("fh_policy_fwd")) return FH_ERR_INJECTED;
+  int rc = policy_check(dtype, rows, vocab, ld, z, actions, stats);
+  if (rc != kOk) return rc;
+  if (!loss || (rows > 0 && (!old || !adv || !lp || (kl_coef != 0.f && !ref))))
+    return fail(FH_ERR_INVALID_ARGUMENT, "policy: old, adv, lp and loss are required, and ref with kl_coef > 0");
+  if (!(clip_low >= 0.f) || !(clip_high >= 0.f) || !(kl_coef >= 0.f) || !(normalizer >= 0.f))
+    return fail(FH_ERR_INVALID_ARGUMENT, "policy: clip_low, clip_high, kl_coef and normalizer must be >= 0");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = select_stream_device(st)) != kOk) return rc;
+  return launch_policy(0,
+                       PolicyArgs{dtype == 1, rows, vocab, ld, z, actions, old, adv, ref, weights, clip_low, clip_high,
+                                  kl_coef, normalizer, lp, loss, stats},
+                       nullptr, nullptr, nullptr, nullptr, st);
+}
+
+static int policy_grad(int op, void* stream, int dtype, int rows, int vocab, long long ld, const void* z,
+                       const long long* actions, const float* stats, const float* g, const void* u, void* out,
+                       float* gg) {
+  int rc = policy_check(dtype, rows, vocab, ld, z, actions, stats);
+  if (rc != kOk || rows == 0) return rc;
+  if (!g || !out || (op == 2 && (!u || !gg)))
+    return fail(FH_ERR_INVALID_ARGUMENT, "policy: g and the outputs (and u) are required");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = select_stream_device(st)) != kOk) return rc;
+  PolicyArgs a{};
+  a.bf16 = dtype == 1;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.ld = ld;
+  a.z = z;
+  a.actions = actions;
+  a.stats = const_cast<float*>(stats);
+  return launch_policy(op, a, g, u, out, gg, st);
+}
+
+int fh_policy_bwd(void* stream, int dtype, int rows, int vocab, long long ld, const void* z, const long long* actions,
+                  const float* stats, const float* g, void* dz) {
+  if (injected("fh_policy_bwd")) return FH_ERR_INJECTED;
+  return policy_grad(1, stream, dtype, rows, vocab, ld, z, actions, stats, g, nullptr, dz, nullptr);
+}
+
+int fh_policy_bwd_bwd(void* stream, int dtype, int rows, int vocab, long long ld, const void* z,
+                      const long long* actions, const float* stats, const float* g, const void* u, void* gz,
+                      float* gg) {
+  if (injected("fh_policy_bwd_bwd")) return FH_ERR_INJECTED;
+  return policy_grad(2, stream, dtype, rows, vocab, ld, z, actions, stats, g, u, gz, gg);
 }
 
 int fh_device_status(void* stream, int* code) {

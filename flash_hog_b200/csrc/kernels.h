@@ -105,6 +105,36 @@ int launch_gelu(int mode, bool bf16, long long n, const void* a, const void* dh,
 int launch_xent(int op, bool bf16, int rows, int vocab, long long ld, const void* z, const long long* t, float* lse,
                 float* loss, const float* g, float s, const void* u, void* out, float* gg, cudaStream_t stream);
 
+// Embedding (embed.cu) of n tokens in a (vocab, dim) table, contiguous, fp32 or bf16.
+// Lookup: y_i = scale w[t_i]; a token outside [0, vocab) gives `oob`, token `skip` zeros.
+// Gradient: dw[v] = scale sum_{t_i = v} dy_i, 0 for `padding` and tokens outside; dw
+// 16-byte aligned; `scratch` 16-byte aligned, embed_scratch_bytes(n, dim).
+int launch_embed_lookup(bool bf16, long long n, int vocab, int dim, const long long* tokens, const void* w,
+                        float scale, long long skip, float oob, void* y, cudaStream_t stream);
+int launch_embed_grad(bool bf16, int n, int vocab, int dim, const long long* tokens, const void* dy, float scale,
+                      long long padding, void* dw, void* scratch, cudaStream_t stream);
+long long embed_scratch_bytes(int n, int dim);
+// Dropout (dropout.cu): y_i = res_i + [u_i >= limit] factor x_i over n elements, u_i the
+// 16-bit draws of (*seed, sub). res may be null. y is bf16 where x and res are, except
+// without a residual, where any pair of types goes.
+int launch_dropout(bool x_bf16, bool res_bf16, bool y_bf16, long long n, const void* x, const void* res, void* y,
+                   const long long* seed, unsigned sub, unsigned limit, float factor, cudaStream_t stream);
+
+// Clipped policy loss (policy.cu): op 0 forward (lp, loss, stats), 1
+// backward (out = dz), 2 backward's backward (u = cotangent of dz; out = gz, gg per row).
+struct PolicyArgs {
+  bool bf16;
+  int rows, vocab;
+  long long ld;
+  const void* z;
+  const long long* actions;
+  const float *old, *adv, *ref, *weights;  // ref: with beta; weights null: all 1
+  float clip_low, clip_high, beta, normalizer;  // normalizer 0: the sum of the weights
+  float *lp, *loss, *stats;  // stats: 6 rows + 1 floats
+};
+int launch_policy(int op, const PolicyArgs& a, const float* g, const void* u, void* out, float* gg,
+                  cudaStream_t stream);
+
 // Checks the kernel launch just made (cudaGetLastError) and, if it was queued,
 // counts it for fh_launch_count(). Returns kOk or kLaunchFailed.
 int after_launch();

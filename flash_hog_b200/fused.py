@@ -1,4 +1,5 @@
-"""LayerNorm, GELU and cross entropy with fused first- and second-order backward kernels.
+"""The ops of a GPT training step around attention, with fused first- and second-order
+backward kernels.
 
 The grad-norm-penalty step (L + lam ||dL/dtheta||^2, configuration 5) differentiates
 every layer's backward once more. In torch autograd the double backward of
@@ -9,6 +10,8 @@ same pattern as the attention op (``flash_hog/jax/attention.py:52-60, 100-130``)
 the outer Function's backward is the inner Function, whose backward is the
 double backward. Third-order derivatives raise.
 
+Embedding and dropout are linear and differentiable to any order.
+
 * ``LayerNorm`` (module) / ``layer_norm(x, w, b, eps)``: fp32 arithmetic; under
   autocast the inputs are cast to fp32, as autocast does for torch's layer_norm.
 * ``gelu(x)``: exact GELU (x Phi(x)) in the input dtype (fp32 or bf16; fp32
@@ -17,6 +20,12 @@ double backward. Third-order derivatives raise.
   (fp32 or bf16, fp32 arithmetic) as ``torch.nn.functional.cross_entropy`` on the
   logits cast to fp32; its gradient comes back in the logits' dtype, as autocast
   would cast it for the head's matmul (``csrc/xent.cu``, ``fh_xent_*``).
+* ``embedding(tokens, weight, scale, padding_idx)`` / ``Embedding`` (module): the scaled
+  lookup, its gradient by sorted tokens (``csrc/embed.cu``, ``fh_embed_*``).
+* ``dropout(x, p, seed, subsequence, residual)``: dropout from a counter-based generator,
+  the mask never stored, with the residual addition (``csrc/dropout.cu``, ``fh_dropout``).
+* ``policy_loss(logits, actions, old_logprobs, advantages, ...)``: the clipped policy loss
+  with a KL term, beside ``cross_entropy`` (``csrc/policy.cu``, ``fh_policy_*``).
 * ``sum_of_squares(tensors)``: the penalty sum_i ||t_i||^2 with torch's multi-tensor
   kernels (one norm pass forward, one scaled copy backward), differentiable once.
 """
@@ -172,6 +181,204 @@ def cross_entropy(logits, targets):
     if logits.stride(-1) != 1:
         logits = logits.contiguous()
     return _CrossEntropy.apply(logits, _contig(targets.long()))
+
+
+class _Embedding(torch.autograd.Function):
+    """scale W[t]; with ``adjoint``, the derivative of ``_EmbeddingBwd`` (zero rows for
+    padding and for tokens outside the table). Linear in W: its backward is
+    ``_EmbeddingBwd``, whose backward is this one again, to any order."""
+
+    @staticmethod
+    def forward(ctx, w, tokens, scale, padding_idx, adjoint):
+        y = torch.empty((*tokens.shape, w.shape[1]), dtype=w.dtype, device=w.device)
+        if adjoint:
+            _capi.embed_bwd_bwd(w, tokens, scale, padding_idx, y)
+        else:
+            _capi.embed_fwd(w, tokens, scale, y)
+        ctx.save_for_backward(tokens)
+        ctx.args = w.shape[0], scale, padding_idx
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        (tokens,) = ctx.saved_tensors
+        return _EmbeddingBwd.apply(dy, tokens, *ctx.args), None, None, None, None
+
+
+class _EmbeddingBwd(torch.autograd.Function):
+    """dW from dy by sorted tokens, every row written."""
+
+    @staticmethod
+    def forward(ctx, dy, tokens, vocab, scale, padding_idx):
+        dy = _contig(dy)
+        dw = torch.empty((vocab, dy.shape[-1]), dtype=dy.dtype, device=dy.device)
+        _capi.embed_bwd(dy, tokens, scale, padding_idx, dw)
+        ctx.save_for_backward(tokens)
+        ctx.args = scale, padding_idx
+        return dw
+
+    @staticmethod
+    def backward(ctx, ddw):
+        (tokens,) = ctx.saved_tensors
+        return _Embedding.apply(_contig(ddw), tokens, *ctx.args, True), None, None, None, None
+
+
+def embedding(tokens, weight, scale: float = 1.0, padding_idx: int | None = None):
+    """``scale * weight[tokens]`` for integer ``tokens`` of any shape and a (vocab, dim)
+    fp32 or bf16 ``weight``, in the weight's dtype; differentiable to any order.
+
+    The gradient sums equal tokens' rows in fp32 in a fixed order (the same result every
+    run) and is zero for ``padding_idx``. A token outside [0, vocab) gives a row of NaN
+    and no gradient.
+    """
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"embedding tokens are int64 or int32, got {tokens.dtype}")
+    if weight.dim() != 2 or weight.dtype not in (torch.float32, torch.bfloat16) or 0 in weight.shape:
+        raise ValueError("the embedding weight is a non-empty (vocab, dim) fp32 or bf16 tensor")
+    if padding_idx is None:
+        padding_idx = -1
+    elif not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError(f"padding_idx must be in [0, {weight.shape[0]}), got {padding_idx}")
+    return _Embedding.apply(_contig(weight), _contig(tokens.long()), float(scale), int(padding_idx), False)
+
+
+class Embedding(nn.Embedding):
+    """``nn.Embedding`` (same parameters and state dict) on the fused kernels, its output
+    multiplied by ``scale``. ``max_norm``, ``scale_grad_by_freq`` and ``sparse`` are refused."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: int | None = None, scale: float = 1.0,
+                 **kwargs):
+        super().__init__(num_embeddings, embedding_dim, padding_idx, **kwargs)
+        if self.max_norm is not None or self.scale_grad_by_freq or self.sparse:
+            raise ValueError("max_norm, scale_grad_by_freq and sparse are not supported")
+        self.scale = float(scale)
+
+    def forward(self, tokens):
+        return embedding(tokens, self.weight, self.scale, self.padding_idx)
+
+
+class _Dropout(torch.autograd.Function):
+    """residual + keep x / (1 - p) in ``dtype``. Linear in x: its backward is itself on dy,
+    with the mask drawn again from the saved seed, to any order."""
+
+    @staticmethod
+    def forward(ctx, x, residual, seed, subsequence, limit, dtype):
+        y = torch.empty(x.shape, dtype=dtype, device=x.device)
+        _capi.dropout(x, residual, y, seed, subsequence, limit)
+        ctx.save_for_backward(seed)
+        ctx.args = subsequence, limit, x.dtype
+        ctx.residual_dtype = None if residual is None else residual.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        (seed,) = ctx.saved_tensors
+        dx = dres = None
+        if ctx.needs_input_grad[0]:
+            dx = _Dropout.apply(_contig(dy), None, seed, *ctx.args)
+        if ctx.needs_input_grad[1]:
+            dres = dy.to(ctx.residual_dtype)
+        return dx, dres, None, None, None, None
+
+
+def dropout(x, p: float, seed, *, subsequence: int = 0, residual=None):
+    """``residual + keep * x / (1 - p)`` (without ``residual``: 0) for fp32 or bf16 tensors,
+    differentiable to any order; in ``x``'s dtype, or with a residual in the promoted one.
+
+    The mask is a function of ``seed``, ``subsequence`` and each element's index in ``x``
+    alone (Philox4x32-10; ``csrc/dropout.cu``) and is drawn again in the backward passes,
+    never stored. ``seed`` is an int64 tensor of one element on ``x``'s device, read when
+    the kernel runs, so a captured graph draws a new mask on replay when its value has
+    changed; it must keep its value until the backward of the same call has run.
+    ``subsequence`` in [0, 2^32) separates calls that share a seed (one per layer). ``p``
+    in [0, 1] is rounded to a multiple of 2^-16; at p = 1 everything is dropped.
+    """
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout p must be in [0, 1], got {p}")
+    if not 0 <= subsequence < 2 ** 32:
+        raise ValueError(f"subsequence must be in [0, 2^32), got {subsequence}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"the residual must have x's shape, got {tuple(residual.shape)} and {tuple(x.shape)}")
+    for t in (x, residual):
+        if t is not None and t.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"dropout takes fp32 or bf16 tensors, got {t.dtype}")
+    dtype = x.dtype if residual is None else torch.promote_types(x.dtype, residual.dtype)
+    return _Dropout.apply(_contig(x), None if residual is None else _contig(residual), seed, int(subsequence),
+                          round(p * 65536), dtype)
+
+
+class _PolicyLossBwd(torch.autograd.Function):
+    """dz = g dloss/dz; its backward is the double backward."""
+
+    @staticmethod
+    def forward(ctx, z, actions, stats, g):
+        g32 = _contig(g.detach().float().reshape(1))
+        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        _capi.policy_bwd(z, actions, stats, g32, dz)
+        ctx.save_for_backward(z, actions, stats, g32)
+        ctx.g_shape, ctx.g_dtype = g.shape, g.dtype
+        return dz
+
+    @staticmethod
+    def backward(ctx, u):
+        z, actions, stats, g32 = ctx.saved_tensors
+        if any(ctx.needs_input_grad) and torch.is_grad_enabled():
+            raise NotImplementedError("third-order derivatives of the fused policy loss are not supported")
+        u = _contig(u.to(z.dtype))
+        gz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        gg = torch.empty(z.shape[0], dtype=torch.float32, device=z.device)
+        _capi.policy_bwd_bwd(z, actions, stats, g32, u, gz, gg)
+        return gz, None, None, gg.sum().to(ctx.g_dtype).reshape(ctx.g_shape)
+
+
+class _PolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, actions, old, adv, ref, weights, clip_low, clip_high, kl_coef, normalizer):
+        rows = z.shape[0]
+        lp = torch.empty(rows, dtype=torch.float32, device=z.device)
+        loss = torch.empty((), dtype=torch.float32, device=z.device)
+        stats = torch.empty(6 * rows + 1, dtype=torch.float32, device=z.device)
+        _capi.policy_fwd(z, actions, old, adv, ref, weights, clip_low, clip_high, kl_coef, normalizer, lp, loss, stats)
+        ctx.save_for_backward(z, actions, stats)
+        ctx.mark_non_differentiable(lp)
+        return loss, lp
+
+    @staticmethod
+    def backward(ctx, g, _g_lp):
+        z, actions, stats = ctx.saved_tensors
+        return (_PolicyLossBwd.apply(z, actions, stats, g),) + (None,) * 9
+
+
+def policy_loss(logits, actions, old_logprobs, advantages, *, ref_logprobs=None, weights=None, clip_low: float = 0.2,
+                clip_high: float = 0.2, kl_coef: float = 0.0, normalizer: float | None = None):
+    """Clipped policy loss with a KL term over (rows, vocab) logits (fp32 or bf16; fp32
+    result), differentiable twice by the logits. Returns ``(loss, logprobs)``.
+
+    Per row, with lp the log probability of ``actions`` under the logits and
+    rho = exp(lp - old_logprobs): -min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) +
+    kl_coef (exp(ref - lp) - (ref - lp) - 1). ``loss`` is the sum of weights * row loss over
+    ``normalizer`` (default: the sum of the weights; 0 where that is 0). Rows of weight 0
+    (prompt, padding) are not read: no loss and no gradient whatever they hold.
+    ``weights`` (default: all 1) may be a boolean mask. Every input but the logits is a
+    constant. ``logprobs`` (fp32, detached) are the lp, 0 in rows of weight 0.
+    An action outside [0, vocab) in a weighted row gives NaN.
+    """
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.shape[1] == 0:
+        raise ValueError("policy_loss takes (rows, vocab) fp32 or bf16 logits")
+    if not (clip_low >= 0.0 and clip_high >= 0.0):
+        raise ValueError("clip_low and clip_high must be >= 0")
+    if not 0.0 <= kl_coef < float("inf"):
+        raise ValueError("kl_coef must be finite and >= 0")
+    if kl_coef > 0.0 and ref_logprobs is None:
+        raise ValueError("kl_coef > 0 needs ref_logprobs")
+    if normalizer is not None and not 0.0 < normalizer < float("inf"):
+        raise ValueError("normalizer must be positive and finite")
+    if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+        logits = logits.contiguous()
+    vec = lambda t: None if t is None else _contig(t.detach().float())
+    return _PolicyLoss.apply(logits, _contig(actions.long()), vec(old_logprobs), vec(advantages),
+                             vec(ref_logprobs) if kl_coef > 0.0 else None, vec(weights), float(clip_low),
+                             float(clip_high), float(kl_coef), 0.0 if normalizer is None else float(normalizer))
 
 
 class _SumOfSquares(torch.autograd.Function):

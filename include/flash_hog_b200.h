@@ -314,6 +314,57 @@ int fh_xent_bwd(void* stream, int dtype, int rows, int vocab, long long ld, cons
 int fh_xent_bwd_bwd(void* stream, int dtype, int rows, int vocab, long long ld, const void* z, const long long* t,
                     const float* lse, const float* g, float s, const void* u, void* gz, float* gg);
 
+/* Embedding of the same model (no counterpart in the reference): a contiguous (vocab,
+ * dim) table w, dtype 0 = fp32, 1 = bf16, and n int64 tokens. Sums and the scaling are
+ * fp32, rounded once to the table's type.
+ *  - fh_embed_fwd: y_i = scale w[t_i], (n, dim); a token outside [0, vocab) gives a row
+ *    of NaN.
+ *  - fh_embed_bwd: dw[v] = scale sum over the i with t_i = v of dy_i, every row written;
+ *    0 for padding_idx (-1: none); tokens outside [0, vocab) contribute nothing. The
+ *    tokens are sorted on the device and equal ones summed in a fixed order: the result
+ *    does not vary from run to run. Three launches. dw and `scratch`
+ *    (fh_embed_scratch_bytes(n, dim) bytes) 16-byte aligned.
+ *  - fh_embed_bwd_bwd: given the cotangent ddw of dw, ddy_i = scale ddw[t_i], 0 for
+ *    padding_idx and tokens outside: the derivative of fh_embed_bwd, which is linear. */
+long long fh_embed_scratch_bytes(int n, int dim);
+int fh_embed_fwd(void* stream, int dtype, int n, int vocab, int dim, const void* w, const long long* tokens,
+                 float scale, void* y);
+int fh_embed_bwd(void* stream, int dtype, int n, int vocab, int dim, const void* dy, const long long* tokens,
+                 float scale, long long padding_idx, void* dw, void* scratch);
+int fh_embed_bwd_bwd(void* stream, int dtype, int n, int vocab, int dim, const void* ddw, const long long* tokens,
+                     float scale, long long padding_idx, void* ddy);
+
+/* Dropout with an optional residual: y_i = res_i + [u_i >= limit] x_i / (1 - limit / 65536)
+ * over n elements; the drop probability is limit / 65536 (limit in [0, 65536]). u_i is
+ * draw i mod 8 (half-words, low half first) of Philox4x32-10 (Salmon et al., 2011) with
+ * key *seed (int64, device memory; low word first) and counter (i / 8 in the first two
+ * words, subsequence, 0). Nothing is stored: the backward is the same call on dy.
+ * dtypes 0 = fp32, 1 = bf16 each; with a residual y is bf16 where x and res are and fp32
+ * otherwise. res may be NULL. fp32 arithmetic, one rounding. */
+int fh_dropout(void* stream, long long n, int x_dtype, const void* x, int res_dtype, const void* res, int y_dtype,
+               void* y, const long long* seed, unsigned int subsequence, int limit);
+
+/* Clipped policy loss with a KL term over logits as in fh_xent_* (rows, vocab, ld, dtype).
+ * Per row: action (int64), old, adv (fp32), ref (fp32, needed where kl_coef > 0) and an
+ * optional weight (fp32; NULL = 1). With lp = z[a] - log sum exp z, rho = exp(lp - old):
+ *   l = -min(rho adv, clip(rho, 1 - clip_low, 1 + clip_high) adv)
+ *       + kl_coef (exp(ref - lp) - (ref - lp) - 1),
+ *   loss = sum w l / N, N = normalizer if that is > 0, else sum w (loss 0 where N = 0).
+ * A row of weight 0 is not read: it gives lp = 0 and zero gradients whatever it holds. An
+ * action outside [0, vocab) in another row gives NaN. rows may be 0.
+ *  - fh_policy_fwd: lp[r], loss[0] and `stats` (6 rows + 1 floats, for the passes below).
+ *  - fh_policy_bwd: dz = g dloss/dz (z's dtype, contiguous); g: fp32, device memory.
+ *  - fh_policy_bwd_bwd: given the cotangent u of dz (z's dtype, contiguous): gz, the
+ *    gradient of <u, dz> by z, and gg[r], whose sum is the one by g. */
+int fh_policy_fwd(void* stream, int dtype, int rows, int vocab, long long ld, const void* z, const long long* actions,
+                  const float* old, const float* adv, const float* ref, const float* weights, float clip_low,
+                  float clip_high, float kl_coef, float normalizer, float* lp, float* loss, float* stats);
+int fh_policy_bwd(void* stream, int dtype, int rows, int vocab, long long ld, const void* z, const long long* actions,
+                  const float* stats, const float* g, void* dz);
+int fh_policy_bwd_bwd(void* stream, int dtype, int rows, int vocab, long long ld, const void* z,
+                      const long long* actions, const float* stats, const float* g, const void* u, void* gz,
+                      float* gg);
+
 /* Synchronises `stream`, then reads and clears the status word the kernels of
  * the current device record device-side failures in. *code receives 0 or one
  * of the device error codes (1..5: which bounded wait expired). Returns FH_OK,
@@ -336,7 +387,7 @@ int fh_abi_version(void);
  * reads it before and after a timed region to report its kernel launches. */
 unsigned long long fh_launch_count(void);
 
-#define FH_ABI_VERSION 8
+#define FH_ABI_VERSION 9
 
 #ifdef __cplusplus
 }
