@@ -39,10 +39,12 @@ class SlidingWindow:
     """A causal mask (``mask_type`` CAUSAL or CAUSAL_BOTTOM_RIGHT) limited to the
     ``length`` keys ending at each query's diagonal -- ``get_mask_bottom_right``'s
     ``qi - kj < sliding_window_length`` (``flash_hog/_jax_refs/jax_impl.py:104-109``).
+    The first ``sinks`` keys stay visible behind the window, up to the diagonal.
     Accepted wherever a ``MaskType`` is."""
 
     mask_type: MaskType
     length: int
+    sinks: int = 0
 
 
 @dataclasses.dataclass(frozen=True, eq=False)
@@ -66,9 +68,16 @@ class PackedSequences:
         return _capi.Varlen(self.cu_seqlens_q, self.cu_seqlens_k, self.max_seqlen_q, self.max_seqlen_k)
 
 
-def _varlen_kw(mask) -> dict:
-    """``{"varlen": ...}`` for the bf16 C ABI wrappers when ``mask`` packs sequences."""
-    return {"varlen": mask.capi()} if isinstance(mask, PackedSequences) else {}
+# Longer windows and sinks than any sequence mean the same; the kernels add them to rows in 32 bits.
+_BAND_MAX = 2 ** 30
+
+
+def _mask_kw(mask) -> dict:
+    """The keyword part of a mask for the C ABI wrappers: ``sinks`` and, for the bf16 ones
+    when ``mask`` packs sequences, ``varlen``."""
+    if isinstance(mask, PackedSequences):
+        return {"varlen": mask.capi(), **_mask_kw(mask.mask)}
+    return {"sinks": min(int(mask.sinks), _BAND_MAX)} if isinstance(mask, SlidingWindow) and mask.sinks else {}
 
 
 def _mask_args(mask) -> tuple[int, int]:
@@ -78,7 +87,9 @@ def _mask_args(mask) -> tuple[int, int]:
     if isinstance(mask, SlidingWindow):
         if mask.mask_type not in (MaskType.CAUSAL, MaskType.CAUSAL_BOTTOM_RIGHT) or mask.length < 1:
             raise ValueError(f"a sliding window needs a causal mask type and a length >= 1, got {mask}")
-        return mask.mask_type.value, int(mask.length)
+        if mask.sinks < 0:
+            raise ValueError(f"a sliding window's sinks must be >= 0, got {mask}")
+        return mask.mask_type.value, min(int(mask.length), _BAND_MAX)
     if not isinstance(mask, MaskType):
         raise ValueError(f"unsupported mask type {mask}")
     return mask.value, 0
@@ -162,9 +173,9 @@ def cuda_dot_product_attention(query, key, value, mask_type: MaskType, scale: fl
     out = torch.empty_like(q)
     lse = torch.empty((b, n, t), dtype=torch.float32, device=q.device)
     if f32:
-        _capi.attn_fwd_f32(q, k, v, out, lse, scale, *_mask_args(mask_type))
+        _capi.attn_fwd_f32(q, k, v, out, lse, scale, *_mask_args(mask_type), **_mask_kw(mask_type))
     else:
-        _capi.attn_fwd(q, k, v, out, lse, scale, *_mask_args(mask_type), **_varlen_kw(mask_type))
+        _capi.attn_fwd(q, k, v, out, lse, scale, *_mask_args(mask_type), **_mask_kw(mask_type))
     out = out.to(query.dtype)
     return (out, lse) if return_residual else out
 
@@ -191,10 +202,10 @@ def dot_product_attention_bwd_rule(mask_type: MaskType, scale: float, res, g, po
     delta = torch.empty((b, n, t), dtype=torch.float32, device=q.device)
     if f32:
         _capi.attn_bwd_f32(q, k, v, o, do, activation.float().contiguous(), dq, dk, dv, delta, scale,
-                           *_mask_args(mask_type))
+                           *_mask_args(mask_type), **_mask_kw(mask_type))
     else:
         _capi.attn_bwd(q, k, v, o, do, activation.float().contiguous(), dq, dk, dv, delta, scale,
-                       *_mask_args(mask_type), **_varlen_kw(mask_type))
+                       *_mask_args(mask_type), **_mask_kw(mask_type))
     return dq.to(query.dtype), dk.to(key.dtype), dv.to(value.dtype)
 
 
@@ -243,11 +254,11 @@ def dot_product_attention_fwd_jvp(mask_type: MaskType, scale: float, res, tangen
     if f32:
         stats = torch.empty((2, b, n, t), dtype=torch.float32, device=q.device)
         _capi.attn_bwdbwd_f32(q, k, v, o, torch.zeros_like(q), tq, tk, tv, lse, None, t_out, None, None, stats[0],
-                              t_lse, stats[1], scale, causal, which=_capi.PASS_QUERY, window=window)
+                              t_lse, stats[1], scale, causal, which=_capi.PASS_QUERY, window=window, **_mask_kw(mask_type))
     else:
         # The forward-tangent pass: the query pass at dO = 0, without the products that vanish there.
         _capi.attn_bwdbwd_o(q, k, v, None, None, tq, tk, tv, lse, None, t_out, None, None, None, t_lse, None, scale,
-                            causal, which=_capi.PASS_FWD_TANGENT, window=window, **_varlen_kw(mask_type))
+                            causal, which=_capi.PASS_FWD_TANGENT, window=window, **_mask_kw(mask_type))
     return t_out.to(out.dtype), t_lse
 
 
@@ -276,7 +287,7 @@ def dot_product_attention_bwd_jvp(mask_type: MaskType, scale: float, res, g, tan
     tdk, tdv = torch.empty_like(k), torch.empty_like(v)
     (_capi.attn_jvp_bwd_f32 if f32 else _capi.attn_jvp_bwd)(
         q, k, v, o, do, activation.float().contiguous(), tq, tk, tv, tdo, tdq, tdk, tdv, t_out,
-        stats[0], stats[1], stats[2], scale, *_mask_args(mask_type), **({} if f32 else _varlen_kw(mask_type)))
+        stats[0], stats[1], stats[2], scale, *_mask_args(mask_type), **_mask_kw(mask_type))
     return tdq.to(query.dtype), tdk.to(key.dtype), tdv.to(value.dtype)
 
 

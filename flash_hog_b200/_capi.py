@@ -97,6 +97,7 @@ class FhAttnDims(ctypes.Structure):
         ("cu_seqlens_k", ctypes.c_void_p),
         ("max_seqlen_q", ctypes.c_int32),
         ("max_seqlen_k", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
     ]
 
 
@@ -176,7 +177,10 @@ def _ptr(t):
 
 
 def _stream(device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    """The current stream of ``device`` (None: of the current device)."""
+    index = torch.cuda.current_device() if device is None or device.index is None else device.index
+    # The handle alone: building a torch.cuda.Stream takes 2-5 us of a call, this 0.1 us.
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))
 
 
 def _on_device(f):
@@ -185,7 +189,7 @@ def _on_device(f):
 
     @functools.wraps(f)
     def call(t, *args, **kwargs):
-        if not t.is_cuda or t.device.index == torch.cuda.current_device():
+        if not t.is_cuda or t.get_device() == torch.cuda.current_device():
             return f(t, *args, **kwargs)
         with torch.cuda.device(t.device):
             return f(t, *args, **kwargs)
@@ -235,13 +239,16 @@ class Varlen:
         return self.cu_seqlens_q.numel() - 1
 
 
-def make_dims(q: torch.Tensor, k: torch.Tensor, window: int = 0, varlen: Varlen | None = None) -> FhAttnDims:
+def make_dims(q: torch.Tensor, k: torch.Tensor, window: int = 0, varlen: Varlen | None = None,
+              sinks: int = 0) -> FhAttnDims:
     """Dims for BTNH tensors: q (B, Tq, H, D), k (B, Tk, Hkv, D) with H a multiple of
-    Hkv; ``window`` is the sliding-window length of a causal mask (0 = unlimited).
+    Hkv; ``window`` is the sliding-window length of a causal mask (0 = unlimited),
+    ``sinks`` the first keys that stay visible behind it.
     With ``varlen`` the tensors are packed (1, total, H, D) sequences."""
     b, tq, h, d = q.shape
     tk, hkv = k.shape[1], k.shape[2]
     dims = FhAttnDims(b, h, tq, tk, d, _strides(q), _strides(k), hkv, int(window))
+    dims.sinks = int(sinks)
     if varlen is not None:
         if b != 1:
             raise ValueError("packed variable-length tensors have one batch entry: (1, total, heads, head_dim)")
@@ -266,14 +273,17 @@ def _same_layout(ref: torch.Tensor, *others: torch.Tensor, dtype=torch.bfloat16)
             raise ValueError(f"tensors must be {dtype} on the same CUDA device")
 
 
-def attn_fwd(q, k, v, out, lse, scale: float, causal: int, window: int = 0, varlen: Varlen | None = None) -> None:
+@_on_device
+def attn_fwd(q, k, v, out, lse, scale: float, causal: int, window: int = 0, varlen: Varlen | None = None,
+             sinks: int = 0) -> None:
     _same_layout(q, out)
     _same_layout(k, v)
-    dims = make_dims(q, k, window, varlen)
+    dims = make_dims(q, k, window, varlen, sinks)
     _check("fh_attn_fwd", lib().fh_attn_fwd(_stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v),
                                            _ptr(out), _ptr(lse), float(scale), int(causal)))
 
 
+@_on_device
 def attn_rowdot(o, dO, delta, varlen: Varlen | None = None) -> None:
     _same_layout(o, dO)
     dims = make_dims(o, o, 0, varlen)
@@ -281,20 +291,24 @@ def attn_rowdot(o, dO, delta, varlen: Varlen | None = None) -> None:
                                                  _ptr(delta)))
 
 
-def attn_bwd(q, k, v, o, dO, lse, dq, dk, dv, delta, scale: float, causal: int, window: int = 0, varlen: Varlen | None = None) -> None:
+@_on_device
+def attn_bwd(q, k, v, o, dO, lse, dq, dk, dv, delta, scale: float, causal: int, window: int = 0, varlen: Varlen | None = None,
+             sinks: int = 0) -> None:
     _same_layout(q, o, dO, dq)
     _same_layout(k, v, dk, dv)
-    dims = make_dims(q, k, window, varlen)
+    dims = make_dims(q, k, window, varlen, sinks)
     _check("fh_attn_bwd", lib().fh_attn_bwd(_stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v),
                                            _ptr(o), _ptr(dO), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv),
                                            _ptr(delta), float(scale), int(causal)))
 
 
+@_on_device
 def attn_bwdbwd(q, k, v, dO, ddq, ddk, ddv, lse, delta, dq2, ddo, dk2, dv2, dd, bvec, scale: float,
-                causal: int, window: int = 0, varlen: Varlen | None = None) -> None:
+                causal: int, window: int = 0, varlen: Varlen | None = None,
+                sinks: int = 0) -> None:
     _same_layout(q, dO, ddq, dq2, ddo)
     _same_layout(k, v, ddk, ddv, dk2, dv2)
-    dims = make_dims(q, k, window, varlen)
+    dims = make_dims(q, k, window, varlen, sinks)
     _check("fh_attn_bwdbwd", lib().fh_attn_bwdbwd(
         _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(dO), _ptr(ddq), _ptr(ddk),
         _ptr(ddv), _ptr(lse), _ptr(delta), _ptr(dq2), _ptr(ddo), _ptr(dk2), _ptr(dv2), _ptr(dd), _ptr(bvec),
@@ -304,36 +318,42 @@ def attn_bwdbwd(q, k, v, dO, ddq, ddk, ddv, lse, delta, dq2, ddo, dk2, dv2, dd, 
 PASS_QUERY, PASS_KEY, PASS_FWD_TANGENT = 1, 2, 4
 
 
+@_on_device
 def attn_bwdbwd_pass(q, k, v, dO, ddq, ddk, ddv, lse, delta, dq2, ddo, dk2, dv2, dd, bvec, scale: float,
-                     causal: int, which: int, window: int = 0, varlen: Varlen | None = None) -> None:
+                     causal: int, which: int, window: int = 0, varlen: Varlen | None = None,
+                     sinks: int = 0) -> None:
     """One pass of the double backward (PASS_QUERY, PASS_KEY or both)."""
     _same_layout(q, dO, ddq, dq2, ddo)
     _same_layout(k, v, ddk, ddv, dk2, dv2)
-    dims = make_dims(q, k, window, varlen)
+    dims = make_dims(q, k, window, varlen, sinks)
     _check("fh_attn_bwdbwd_pass", lib().fh_attn_bwdbwd_pass(
         _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(dO), _ptr(ddq), _ptr(ddk),
         _ptr(ddv), _ptr(lse), _ptr(delta), _ptr(dq2), _ptr(ddo), _ptr(dk2), _ptr(dv2), _ptr(dd), _ptr(bvec),
         float(scale), int(causal), int(which)))
 
 
+@_on_device
 def attn_bwdbwd_o(q, k, v, o, dO, ddq, ddk, ddv, lse, dq2, ddo, dk2, dv2, delta, dd, bvec, scale: float,
-                  causal: int, which: int = PASS_QUERY | PASS_KEY, window: int = 0, varlen: Varlen | None = None) -> None:
+                  causal: int, which: int = PASS_QUERY | PASS_KEY, window: int = 0, varlen: Varlen | None = None,
+                  sinks: int = 0) -> None:
     """Double backward from the forward output: the query pass computes delta itself."""
     _same_layout(q, o, dO, ddq, dq2, ddo)
     _same_layout(k, v, ddk, ddv, dk2, dv2)
-    dims = make_dims(q, k, window, varlen)
+    dims = make_dims(q, k, window, varlen, sinks)
     _check("fh_attn_bwdbwd_o", lib().fh_attn_bwdbwd_o(
         _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dO), _ptr(ddq),
         _ptr(ddk), _ptr(ddv), _ptr(lse), _ptr(dq2), _ptr(ddo), _ptr(dk2), _ptr(dv2), _ptr(delta), _ptr(dd),
         _ptr(bvec), float(scale), int(causal), int(which)))
 
 
+@_on_device
 def attn_jvp_bwd(q, k, v, o, dO, lse, tq, tk, tv, tdO, tdq, tdk, tdv, to, delta, dd, bvec, scale: float,
-                 causal: int, window: int = 0, varlen: Varlen | None = None) -> None:
+                 causal: int, window: int = 0, varlen: Varlen | None = None,
+                 sinks: int = 0) -> None:
     """Forward-mode derivative of the first-order backward (``tdO`` may be None)."""
     _same_layout(q, o, dO, tq, tdq, to, tdO)
     _same_layout(k, v, tk, tv, tdk, tdv)
-    dims = make_dims(q, k, window, varlen)
+    dims = make_dims(q, k, window, varlen, sinks)
     _check("fh_attn_jvp_bwd", lib().fh_attn_jvp_bwd(
         _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dO), _ptr(lse), _ptr(tq),
         _ptr(tk), _ptr(tv), _ptr(tdO), _ptr(tdq), _ptr(tdk), _ptr(tdv), _ptr(to),
@@ -343,43 +363,47 @@ def attn_jvp_bwd(q, k, v, o, dO, lse, tq, tk, tv, tdO, tdq, tdk, tdv, to, delta,
 _F32 = torch.float32
 
 
-def attn_fwd_f32(q, k, v, out, lse, scale: float, causal: int, window: int = 0) -> None:
+@_on_device
+def attn_fwd_f32(q, k, v, out, lse, scale: float, causal: int, window: int = 0, sinks: int = 0) -> None:
     """``attn_fwd`` with fp32 tensors, fp32 products (``fh_attn_fwd_f32``)."""
     _same_layout(q, out, dtype=_F32)
     _same_layout(k, v, dtype=_F32)
-    dims = make_dims(q, k, window)
+    dims = make_dims(q, k, window, None, sinks)
     _check("fh_attn_fwd_f32", lib().fh_attn_fwd_f32(_stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k),
                                                    _ptr(v), _ptr(out), _ptr(lse), float(scale), int(causal)))
 
 
-def attn_bwd_f32(q, k, v, o, dO, lse, dq, dk, dv, delta, scale: float, causal: int, window: int = 0) -> None:
+@_on_device
+def attn_bwd_f32(q, k, v, o, dO, lse, dq, dk, dv, delta, scale: float, causal: int, window: int = 0, sinks: int = 0) -> None:
     """``attn_bwd`` with fp32 tensors (``fh_attn_bwd_f32``)."""
     _same_layout(q, o, dO, dq, dtype=_F32)
     _same_layout(k, v, dk, dv, dtype=_F32)
-    dims = make_dims(q, k, window)
+    dims = make_dims(q, k, window, None, sinks)
     _check("fh_attn_bwd_f32", lib().fh_attn_bwd_f32(_stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k),
                                                    _ptr(v), _ptr(o), _ptr(dO), _ptr(lse), _ptr(dq), _ptr(dk),
                                                    _ptr(dv), _ptr(delta), float(scale), int(causal)))
 
 
+@_on_device
 def attn_bwdbwd_f32(q, k, v, o, dO, ddq, ddk, ddv, lse, dq2, ddo, dk2, dv2, delta, dd, bvec, scale: float,
-                    causal: int, which: int = PASS_QUERY | PASS_KEY, window: int = 0) -> None:
+                    causal: int, which: int = PASS_QUERY | PASS_KEY, window: int = 0, sinks: int = 0) -> None:
     """``attn_bwdbwd_o`` with fp32 tensors (``fh_attn_bwdbwd_f32``)."""
     _same_layout(q, o, dO, ddq, dq2, ddo, dtype=_F32)
     _same_layout(k, v, ddk, ddv, dk2, dv2, dtype=_F32)
-    dims = make_dims(q, k, window)
+    dims = make_dims(q, k, window, None, sinks)
     _check("fh_attn_bwdbwd_f32", lib().fh_attn_bwdbwd_f32(
         _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dO), _ptr(ddq),
         _ptr(ddk), _ptr(ddv), _ptr(lse), _ptr(dq2), _ptr(ddo), _ptr(dk2), _ptr(dv2), _ptr(delta), _ptr(dd),
         _ptr(bvec), float(scale), int(causal), int(which)))
 
 
+@_on_device
 def attn_jvp_bwd_f32(q, k, v, o, dO, lse, tq, tk, tv, tdO, tdq, tdk, tdv, to, delta, dd, bvec, scale: float,
-                     causal: int, window: int = 0) -> None:
+                     causal: int, window: int = 0, sinks: int = 0) -> None:
     """``attn_jvp_bwd`` with fp32 tensors (``fh_attn_jvp_bwd_f32``)."""
     _same_layout(q, o, dO, tq, tdq, to, tdO, dtype=_F32)
     _same_layout(k, v, tk, tv, tdk, tdv, dtype=_F32)
-    dims = make_dims(q, k, window)
+    dims = make_dims(q, k, window, None, sinks)
     _check("fh_attn_jvp_bwd_f32", lib().fh_attn_jvp_bwd_f32(
         _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dO), _ptr(lse), _ptr(tq),
         _ptr(tk), _ptr(tv), _ptr(tdO), _ptr(tdq), _ptr(tdk), _ptr(tdv), _ptr(to),

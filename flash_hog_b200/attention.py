@@ -37,8 +37,25 @@ from flash_hog_b200 import _attention_impl as attn_impl
 from flash_hog_b200._attention_impl import MaskType, PackedSequences, SlidingWindow
 
 
+def _mask_of(is_causal, causal_alignment, sliding_window_length, sink_tokens):
+    """The MaskType or SlidingWindow of the keyword arguments of the two entry points."""
+    if causal_alignment not in ("top_left", "bottom_right"):
+        raise ValueError(f"causal_alignment must be 'top_left' or 'bottom_right', got {causal_alignment!r}")
+    if not is_causal and (sliding_window_length is not None or causal_alignment != "top_left"):
+        raise ValueError("causal_alignment and sliding_window_length apply to causal attention only")
+    if sink_tokens != 0 and sliding_window_length is None:
+        raise ValueError("sink_tokens apply to a sliding window: sliding_window_length is not given")
+    if not is_causal:
+        return MaskType.NO_MASK
+    mask_type = MaskType.CAUSAL if causal_alignment == "top_left" else MaskType.CAUSAL_BOTTOM_RIGHT
+    if sliding_window_length is not None:
+        mask_type = SlidingWindow(mask_type, int(sliding_window_length), int(sink_tokens))
+    return mask_type
+
+
 def dot_product_attention(query, key, value, is_causal: bool = False, scale: float | None = None, *,
-                          causal_alignment: str = "top_left", sliding_window_length: int | None = None):
+                          causal_alignment: str = "top_left", sliding_window_length: int | None = None,
+                          sink_tokens: int = 0):
     """softmax(scale * query key^T [+ causal mask]) value.
 
     Dimensions: T query length, S key/value length, N heads, H head dim.
@@ -48,22 +65,16 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
     ``causal_alignment`` "top_left" (query i sees keys j <= i, the reference API's
     mask) or "bottom_right" (j <= i + S - T, the alignment of the reference's JAX
     statements, ``flash_hog/_jax_refs/jax_impl.py:104-109``), and
-    ``sliding_window_length`` W (each query sees the W keys ending at its diagonal).
+    ``sliding_window_length`` W (each query sees the W keys ending at its diagonal) and,
+    with a window, ``sink_tokens`` S (the first S keys stay visible behind it: query i
+    sees key j iff j <= diag_i and (j > diag_i - W or j < S)).
     A query that sees no key gets a zero output.
     """
     if scale is None:
         scale = query.shape[-1] ** -0.5
     if not (query.dtype == key.dtype == value.dtype):
         raise TypeError("query, key and value must share a dtype")
-    if causal_alignment not in ("top_left", "bottom_right"):
-        raise ValueError(f"causal_alignment must be 'top_left' or 'bottom_right', got {causal_alignment!r}")
-    if not is_causal and (sliding_window_length is not None or causal_alignment != "top_left"):
-        raise ValueError("causal_alignment and sliding_window_length apply to causal attention only")
-    mask_type = MaskType.NO_MASK
-    if is_causal:
-        mask_type = MaskType.CAUSAL if causal_alignment == "top_left" else MaskType.CAUSAL_BOTTOM_RIGHT
-        if sliding_window_length is not None:
-            mask_type = SlidingWindow(mask_type, int(sliding_window_length))
+    mask_type = _mask_of(is_causal, causal_alignment, sliding_window_length, sink_tokens)
     unbatched = query.ndim == 3
     if unbatched:
         query, key, value = query.unsqueeze(0), key.unsqueeze(0), value.unsqueeze(0)
@@ -77,7 +88,8 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
 
 def dot_product_attention_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, max_seqlen_q: int,
                                  max_seqlen_k: int, is_causal: bool = False, scale: float | None = None, *,
-                                 causal_alignment: str = "top_left", sliding_window_length: int | None = None):
+                                 causal_alignment: str = "top_left", sliding_window_length: int | None = None,
+                                 sink_tokens: int = 0):
     """``dot_product_attention`` over a packed batch of variable-length sequences,
     differentiable twice like it (fwd -> bwd -> bwdbwd on the kernels).
 
@@ -87,7 +99,8 @@ def dot_product_attention_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, 
     non-decreasing from 0); ``max_seqlen_q``/``max_seqlen_k`` bound the lengths. Masks
     apply per sequence: "bottom_right" aligns each sequence's own diagonal, the mask of
     the reference's JAX statements for a (qs, ks) pair
-    (``flash_hog/_jax_refs/jax_impl.py:104-130``). Each sequence's result equals the
+    (``flash_hog/_jax_refs/jax_impl.py:104-130``); ``sink_tokens`` are the first keys of
+    each sequence. Each sequence's result equals the
     dense call on that sequence alone. Computes with bf16 operands (any input dtype;
     results in the input dtype).
     """
@@ -95,15 +108,7 @@ def dot_product_attention_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, 
         raise ValueError("packed tensors are (total, heads, head_dim)")
     if scale is None:
         scale = query.shape[-1] ** -0.5
-    if causal_alignment not in ("top_left", "bottom_right"):
-        raise ValueError(f"causal_alignment must be 'top_left' or 'bottom_right', got {causal_alignment!r}")
-    if not is_causal and (sliding_window_length is not None or causal_alignment != "top_left"):
-        raise ValueError("causal_alignment and sliding_window_length apply to causal attention only")
-    mask = MaskType.NO_MASK
-    if is_causal:
-        mask = MaskType.CAUSAL if causal_alignment == "top_left" else MaskType.CAUSAL_BOTTOM_RIGHT
-        if sliding_window_length is not None:
-            mask = SlidingWindow(mask, int(sliding_window_length))
+    mask = _mask_of(is_causal, causal_alignment, sliding_window_length, sink_tokens)
     packed = PackedSequences(mask, cu_seqlens_q, cu_seqlens_k, int(max_seqlen_q), int(max_seqlen_k))
     result, _ = _DotProductAttention.apply(query.unsqueeze(0), key.unsqueeze(0), value.unsqueeze(0), packed,
                                            float(scale), "bf16")

@@ -22,7 +22,7 @@ import torch
 
 from flash_hog_b200 import _capi
 from flash_hog_b200._attention_impl import (MaskType, PackedSequences, _fold, _is_f32, _mask_args, _operand, _unfold,
-                                            _varlen_kw, fp32_policy)
+                                            _mask_kw, fp32_policy)
 
 
 @dataclasses.dataclass(frozen=True)
@@ -66,7 +66,7 @@ def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, mask_type: MaskType = MaskTyp
     policy = fp32_policy() if _policy is None else _policy
     packed = mask_type if isinstance(mask_type, PackedSequences) else None
     dq2, dk2, dv2, ddo, stats = _FlashBwdBwd.apply(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal, window, float(scale),
-                                                   policy, packed)
+                                                   policy, packed, _mask_kw(mask_type).get("sinks", 0))
     outs = (dq2, dk2, dv2, ddo)
     if return_stats:
         return outs, (stats[0], stats[1], stats[2])
@@ -74,7 +74,7 @@ def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, mask_type: MaskType = MaskTyp
 
 
 def _bwdbwd_device(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal: int, window: int, scale: float, policy: str,
-                   packed: PackedSequences | None = None):
+                   packed: PackedSequences | None = None, sinks: int = 0):
     """The kernels on 4-D BTNH tensors: ``(dQ2, dK2, dV2, ddO, stats)``, stats = (D, dD, B) stacked.
     ``packed``: the tensors are (1, total, heads, head_dim) packed sequences."""
     f32 = _is_f32(Q, policy, packed)
@@ -88,7 +88,7 @@ def _bwdbwd_device(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal: int, window: int, s
     # D = rowsum(dO * O) is computed on the device as part of the call.
     entry = _capi.attn_bwdbwd_f32 if f32 else _capi.attn_bwdbwd_o
     entry(q, k, v, o, do, ddq, ddk, ddv, lse, dq2, ddo, dk2, dv2, delta, dd, bvec, scale, causal, window=window,
-          **({} if f32 else _varlen_kw(packed)))
+          **{**_mask_kw(packed), "sinks": sinks})
     return dq2.to(Q.dtype), dk2.to(K.dtype), dv2.to(V.dtype), ddo.to(dO.dtype), stats
 
 
@@ -98,8 +98,9 @@ class _FlashBwdBwd(torch.autograd.Function):
     Returns ``(dQ2, dK2, dV2, ddO, stats)``."""
 
     @staticmethod
-    def forward(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal, window, scale, policy, packed):
-        return _bwdbwd_device(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal, window, scale, policy, packed)
+    def forward(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal, window, scale, policy, packed, sinks):
+        return _bwdbwd_device(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal, window, scale, policy, packed,
+                              **({"sinks": sinks} if sinks else {}))
 
     @staticmethod
     def setup_context(ctx, inputs, output):
@@ -112,7 +113,7 @@ class _FlashBwdBwd(torch.autograd.Function):
             "reference's double-backward rule is the last one it defines, flash_hog/jax/attention.py:100-130)")
 
     @staticmethod
-    def vmap(info, in_dims, Q, K, V, O, dO, ddQ, ddK, ddV, L, causal, window, scale, policy, packed):
+    def vmap(info, in_dims, Q, K, V, O, dO, ddQ, ddK, ddV, L, causal, window, scale, policy, packed, sinks):
         """Batching rule of ``flash_hog/jax/_pallas_gpu.py:85-102``: the vmapped axis is
         folded into the batch axis, the kernels run once, and the results are unfolded.
         The reference requires every input to be vmapped; here an input that is not is
@@ -121,7 +122,7 @@ class _FlashBwdBwd(torch.autograd.Function):
             raise NotImplementedError("packed variable-length batches are not vmapped: pack the sequences instead")
         size = info.batch_size
         args = [_fold(x, d, size) for x, d in zip((Q, K, V, O, dO, ddQ, ddK, ddV, L), in_dims[:9])]
-        dq2, dk2, dv2, ddo, stats = _FlashBwdBwd.apply(*args, causal, window, scale, policy, None)
+        dq2, dk2, dv2, ddo, stats = _FlashBwdBwd.apply(*args, causal, window, scale, policy, None, sinks)
         stats = stats.reshape(3, size, stats.shape[1] // size, *stats.shape[2:])
         return (_unfold(dq2, size), _unfold(dk2, size), _unfold(dv2, size), _unfold(ddo, size), stats), (0, 0, 0, 0, 1)
 

@@ -42,6 +42,9 @@ struct Strides3 {
 // Tk - Tq: bottom-right; window: sliding-window length). Without `causal` every
 // key is visible.
 //
+// With window > 0, sinks > 0 keeps the first `sinks` keys visible behind the window:
+// query i also sees key j < sinks where j <= i + diag.
+//
 // Packed variable-length batches: with cu_q/cu_k set, sequence b is rows
 // [cu_q[b], cu_q[b+1]) of the packed query-side tensors (batch 1, total_q rows)
 // and rows [cu_k[b], cu_k[b+1]) of the key-side ones; Tq/Tk are then the longest
@@ -61,6 +64,7 @@ struct AttnShape {
   const int* cu_q;            // varlen sequence starts (B + 1 entries), or null (dense)
   const int* cu_k;
   int total_q, total_k;       // rows of the packed tensors (varlen); Tq, Tk (dense)
+  int sinks;                  // first keys that a window leaves visible (0 without a window)
 };
 
 // Where sequence b's rows start: the batch coordinate of its tensors' views and
@@ -90,7 +94,7 @@ __device__ __forceinline__ AttnShape seq_shape(const AttnShape& s, int b, SeqRan
   return l;
 }
 
-// Visible keys [key_lo, key_hi] of query row i (empty when key_hi < key_lo).
+// Visible keys [key_lo, key_hi] of query row i (empty when key_hi < key_lo), sinks aside.
 __host__ __device__ __forceinline__ int key_hi(const AttnShape& s, int i) {
   return s.causal ? min(s.Tk - 1, i + s.diag) : s.Tk - 1;
 }
@@ -102,7 +106,7 @@ __host__ __device__ __forceinline__ int query_lo(const AttnShape& s, int j) {
   return s.causal ? max(0, j - s.diag) : 0;
 }
 __host__ __device__ __forceinline__ int query_hi(const AttnShape& s, int j) {
-  return (s.causal && s.window > 0) ? min(s.Tq - 1, j - s.diag + s.window - 1) : s.Tq - 1;
+  return (s.causal && s.window > 0 && j >= s.sinks) ? min(s.Tq - 1, j - s.diag + s.window - 1) : s.Tq - 1;
 }
 
 // Streamed tiles of `bn` rows that query rows [r0, r0 + rows) need: tiles
@@ -116,12 +120,39 @@ __host__ __device__ __forceinline__ int key_tiles(const AttnShape& s, int r0, in
   *first = lo / bn;
   return hi / bn + 1 - *first;
 }
+// The key tiles of query rows [r0, r0 + rows) with sinks (or without any): the tiles of
+// the sinks, then those of the window, as one list of n tiles of which number `it` is key
+// tile tile(it). The two parts are one run where they touch.
+struct SinkTiles {
+  int n, split, jump;  // from entry `split` on the window's tiles, `jump` further
+  __host__ __device__ __forceinline__ int tile(int it) const { return it < split ? it : it + jump; }
+};
+__host__ __device__ __forceinline__ SinkTiles sink_key_tiles(const AttnShape& s, int r0, int rows, int bn) {
+  SinkTiles t{0, 0, 0};
+  const int r1 = min(r0 + rows, s.Tq) - 1;
+  if (r1 < r0) return t;
+  const int lo = key_lo(s, r0), hi = key_hi(s, r1);
+  if (hi < 0) return t;
+  const int front = (min(s.sinks, hi + 1) + bn - 1) / bn, first = lo / bn, end = hi / bn + 1;
+  if (hi < lo) {  // past the keys' window: the sinks alone
+    t.n = t.split = front;
+  } else if (first <= front) {
+    t.n = t.split = end;
+  } else {
+    t.n = front + end - first;
+    t.split = front;
+    t.jump = first - front;
+  }
+  return t;
+}
+
 // Streamed tiles of `bn` query rows that key rows [k0, k0 + rows) need.
 __host__ __device__ __forceinline__ int query_tiles(const AttnShape& s, int k0, int rows, int bn, int* first) {
   const int k1 = min(k0 + rows, s.Tk) - 1;
   *first = 0;
   if (k1 < k0) return 0;
-  const int lo = query_lo(s, k0), hi = query_hi(s, k1);
+  // A tile that holds a sink is seen by every query from its first key's on.
+  const int lo = query_lo(s, k0), hi = k0 < s.sinks ? s.Tq - 1 : query_hi(s, k1);
   if (hi < lo) return 0;
   *first = lo / bn;
   return hi / bn + 1 - *first;

@@ -87,23 +87,25 @@ struct DqPass {
 
 // Packed bf16 pairs of dS/scale = P (dP - D) for this thread's CW key columns
 // (column pairs through the packed fp32x2 instructions).
-template <int CW, bool MASK>
+// MASK: 0 every key visible, 1 those of [klo, khi], 2 those and the first `snk` up to khi.
+template <int CW, int MASK>
 __device__ __forceinline__ void dq_ops(const uint32_t (&vs)[CW], const uint32_t (&vdp)[CW], int kc, int klo, int khi,
-                                       float sc2, float lg, float dv, uint32_t (&o_ds)[CW / 2]) {
+                                       int snk, float sc2, float lg, float dv, uint32_t (&o_ds)[CW / 2]) {
   const float2 m = make_float2(sc2, sc2), nl = make_float2(-lg, -lg), ndv = make_float2(-dv, -dv);
 #pragma unroll
   for (int i = 0; i < CW; i += 2) {
     float2 s = __ffma2_rn(f2(vs[i], vs[i + 1]), m, nl);
     if (MASK) {
-      if (kc + i > khi || kc + i < klo) s.x = -INFINITY;
-      if (kc + i + 1 > khi || kc + i + 1 < klo) s.y = -INFINITY;
+      if (kc + i > khi || (kc + i < klo && (MASK == 1 || kc + i >= snk))) s.x = -INFINITY;
+      if (kc + i + 1 > khi || (kc + i + 1 < klo && (MASK == 1 || kc + i + 1 >= snk))) s.y = -INFINITY;
     }
     const float2 ds = __fmul2_rn(make_float2(ex2(s.x), ex2(s.y)), __fadd2_rn(f2(vdp[i], vdp[i + 1]), ndv));
     o_ds[i / 2] = pack_bf16(ds.x, ds.y);
   }
 }
 
-template <int HD, bool VL, bool GRP>
+// SNK: a window with sinks (the key tiles are SinkTiles).
+template <int HD, bool VL, bool GRP, bool SNK>
 __global__ void __launch_bounds__(kBBThreads, DqPass<HD>::CTAS)
     bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                   const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -140,7 +142,15 @@ __global__ void __launch_bounds__(kBBThreads, DqPass<HD>::CTAS)
   const AttnShape sh = seq_shape<VL>(a.sh, b, &sr);  // this sequence's lengths and mask; sr: where its rows start
   const int q0 = qt * kBM;
   int j0;
-  const int n = key_tiles(sh, q0, kBM, BN, &j0);  // key tiles j0, j0 + 1, ... (0: no row sees a key)
+  int n = 0;  // key tiles j0, j0 + 1, ... or, with sinks, sink.tile(0), ... (0: no row sees a key)
+  SinkTiles sink{0, 0, 0};
+  if constexpr (SNK) {
+    sink = sink_key_tiles(sh, q0, kBM, BN);
+    n = sink.n;
+  } else {
+    n = key_tiles(sh, q0, kBM, BN, &j0);
+  }
+  auto key_row = [&](int it) { return (SNK ? sink.tile(it) : j0 + it) * BN; };  // first key of tile `it`
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -188,8 +198,8 @@ __global__ void __launch_bounds__(kBBThreads, DqPass<HD>::CTAS)
         }
         uint8_t* slot = s_ring + s * G::SLOT;
         mbar_arrive_expect_tx(&bar_full[s], G::SLOT);
-        tma_rows<HD>(slot, &tm_k, &bar_full[s], sr.k0 + (j0 + it) * BN, BN, h / sh.G, sr.bc);
-        tma_rows<HD>(slot + G::STR, &tm_v, &bar_full[s], sr.k0 + (j0 + it) * BN, BN, h / sh.G, sr.bc);
+        tma_rows<HD>(slot, &tm_k, &bar_full[s], sr.k0 + key_row(it), BN, h / sh.G, sr.bc);
+        tma_rows<HD>(slot + G::STR, &tm_v, &bar_full[s], sr.k0 + key_row(it), BN, h / sh.G, sr.bc);
         issued = it + 1;
       }
       // Every issued copy must land before this CTA's shared memory is released.
@@ -292,13 +302,13 @@ __global__ void __launch_bounds__(kBBThreads, DqPass<HD>::CTAS)
         reg_fence(vs);
         reg_fence(vdp);
         warp_arrive(&bar_sc_empty[wg]);  // the tensor core may reuse this score buffer now
-        const int kc = (j0 + j) * BN;
-        const bool need_mask = kc + BN - 1 > khi || kc < klo;
+        const int kc = key_row(j);
+        const bool need_mask = kc + BN - 1 > khi || (kc < klo && (!SNK || kc + BN > sh.sinks));
         uint32_t o_ds[BN / 2];
         if (need_mask)
-          dq_ops<BN, true>(vs, vdp, kc, klo, khi, sc2, lg, dv, o_ds);
+          dq_ops<BN, SNK ? 2 : 1>(vs, vdp, kc, klo, khi, sh.sinks, sc2, lg, dv, o_ds);
         else
-          dq_ops<BN, false>(vs, vdp, kc, klo, khi, sc2, lg, dv, o_ds);
+          dq_ops<BN, 0>(vs, vdp, kc, klo, khi, 0, sc2, lg, dv, o_ds);
         if (u > 0) ok = mbar_wait_warp(&bar_ops_empty[wg], (u - 1) & 1, &abort_flag);
         if (!ok) break;
         tc_fence_after();
@@ -322,13 +332,13 @@ __global__ void __launch_bounds__(kBBThreads, DqPass<HD>::CTAS)
         reg_fence(vs);
         reg_fence(vdp);
         warp_arrive(&bar_sc_empty[0]);
-        const int kc = (j0 + j) * BN + cb;  // first key of this thread's columns
-        const bool need_mask = kc + CW - 1 > khi || kc < klo;
+        const int kc = key_row(j) + cb;  // first key of this thread's columns
+        const bool need_mask = kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sh.sinks));
         uint32_t o_ds[CW / 2];
         if (need_mask)
-          dq_ops<CW, true>(vs, vdp, kc, klo, khi, sc2, lg, dv, o_ds);
+          dq_ops<CW, SNK ? 2 : 1>(vs, vdp, kc, klo, khi, sh.sinks, sc2, lg, dv, o_ds);
         else
-          dq_ops<CW, false>(vs, vdp, kc, klo, khi, sc2, lg, dv, o_ds);
+          dq_ops<CW, 0>(vs, vdp, kc, klo, khi, 0, sc2, lg, dv, o_ds);
         if (j > 0) ok = mbar_wait_warp(&bar_ops_empty[0], (j - 1) & 1, &abort_flag);
         if (!ok) break;
         tc_fence_after();
@@ -748,14 +758,6 @@ int launch_bwd_hd(const AttnShape& s, const BwdPtrs& p, int* status, cudaStream_
             make_seq_map(&mk[2], p.q, HD, s.total_q, s.H, map_batch(s), s.sq, GK::BN) &&
             make_seq_map(&mk[3], p.dO, HD, s.total_q, s.H, map_batch(s), s.sq, GK::BN);
   if (!ok) return kInvalidArgument;
-  if (ensure_smem_limit(reinterpret_cast<const void*>(&bwd_dq_kernel<HD, VL, false>), GQ::SMEM) != kOk ||
-      ensure_smem_limit(reinterpret_cast<const void*>(&bwd_dkdv_kernel<HD, VL, false>), GK::SMEM) != kOk)
-    return kLaunchFailed;
-  if constexpr (!VL) {
-    if (ensure_smem_limit(reinterpret_cast<const void*>(&bwd_dq_kernel<HD, false, true>), GQ::SMEM) != kOk ||
-        ensure_smem_limit(reinterpret_cast<const void*>(&bwd_dkdv_kernel<HD, false, true>), GK::SMEM) != kOk)
-      return kLaunchFailed;
-  }
   BwdArgs args{s,
                p.lse,
                p.delta,
@@ -770,22 +772,36 @@ int launch_bwd_hd(const AttnShape& s, const BwdPtrs& p, int* status, cudaStream_
                // dO of its query heads (dK/dV pass).
                locality_group(s.H * s.B, s.H / s.Hk, 2ll * s.Tk * HD * 2),
                locality_group(s.Hk * s.B, 1, 2ll * (s.H / s.Hk) * s.Tq * HD * 2)};
-  // The grouped kernels only where the groups split the pairs.
   const int nq = (s.Tq + kBM - 1) / kBM, nk = (s.Tk + kBM - 1) / kBM;
-  if (!VL && args.grp_q < s.H * s.B)
-    bwd_dq_kernel<HD, false, true><<<dim3(s.H * s.B * nq), kBBThreads, GQ::SMEM, stream>>>(mq[0], mq[1], mq[2], mq[3],
-                                                                                         mq[4], args);
-  else
-    bwd_dq_kernel<HD, VL, false><<<dim3(s.H, s.B, nq), kBBThreads, GQ::SMEM, stream>>>(mq[0], mq[1], mq[2], mq[3],
-                                                                                     mq[4], args);
-  if (after_launch() != kOk) return kLaunchFailed;
-  if (!VL && args.grp_k < s.Hk * s.B)
-    bwd_dkdv_kernel<HD, false, true><<<dim3(s.Hk * s.B * nk), kBBThreads, GK::SMEM, stream>>>(mk[0], mk[1], mk[2],
-                                                                                            mk[3], args);
-  else
-    bwd_dkdv_kernel<HD, VL, false><<<dim3(s.Hk, s.B, nk), kBBThreads, GK::SMEM, stream>>>(mk[0], mk[1], mk[2], mk[3],
-                                                                                        args);
-  return after_launch();
+  auto launch_q = [&](auto* kernel, dim3 grid) {
+    if (ensure_smem_limit(reinterpret_cast<const void*>(kernel), GQ::SMEM) != kOk) return kLaunchFailed;
+    kernel<<<grid, kBBThreads, GQ::SMEM, stream>>>(mq[0], mq[1], mq[2], mq[3], mq[4], args);
+    return static_cast<HostStatus>(after_launch());
+  };
+  auto launch_k = [&](auto* kernel, dim3 grid) {
+    if (ensure_smem_limit(reinterpret_cast<const void*>(kernel), GK::SMEM) != kOk) return kLaunchFailed;
+    kernel<<<grid, kBBThreads, GK::SMEM, stream>>>(mk[0], mk[1], mk[2], mk[3], args);
+    return static_cast<HostStatus>(after_launch());
+  };
+  // The grouped kernels only where the groups split the pairs, and not with sinks: their
+  // query tiles share few of their keys.
+  const dim3 grid_q(s.H, s.B, nq), grid_k(s.Hk, s.B, nk);
+  HostStatus rc = kOk;
+  bool done = false;
+  if constexpr (!VL) {
+    if (s.sinks == 0 && args.grp_q < s.H * s.B) {
+      rc = launch_q(&bwd_dq_kernel<HD, false, true, false>, dim3(s.H * s.B * nq));
+      done = true;
+    }
+  }
+  if (!done)
+    rc = s.sinks > 0 ? launch_q(&bwd_dq_kernel<HD, VL, false, true>, grid_q)
+                     : launch_q(&bwd_dq_kernel<HD, VL, false, false>, grid_q);
+  if (rc != kOk) return rc;
+  if constexpr (!VL) {
+    if (args.grp_k < s.Hk * s.B) return launch_k(&bwd_dkdv_kernel<HD, false, true>, dim3(s.Hk * s.B * nk));
+  }
+  return launch_k(&bwd_dkdv_kernel<HD, VL, false>, grid_k);
 }
 
 }  // namespace

@@ -85,24 +85,27 @@ struct QPass {
   static_assert(CW % 16 == 0 && HD % 64 == 0, "tile shapes");
 };
 
+// MASK of the four element-wise forms below: 0 every key visible, 1 those of [klo, khi],
+// 2 those and the first `snk` up to khi.
+
 // Stats sweep: row partial sums over this thread's CW columns. dD and r3 are
 // accumulated without the softmax scale of ddS (applied once per row after the
 // sweep): dD/scale += P ddS', r1 += P dPa, r2 += P dP, r3/scale += P ddS' dP.
 // The arithmetic runs on column pairs with the packed fp32x2 instructions
 // (fma/mul/add.rn.f32x2: per lane the same IEEE results as the scalar forms, one
 // issue slot for two), so the sums are kept as (even, odd) column pairs.
-template <int CW, bool MASK>
+template <int CW, int MASK>
 __device__ __forceinline__ void q_stats(const uint32_t (&vs)[CW], const uint32_t (&vdds)[CW],
                                         const uint32_t (&vdp)[CW], const uint32_t (&vdpa)[CW], int kc, int klo,
-                                        int khi, float sc2, float lg, float2& dD, float2& r1, float2& r2,
+                                        int khi, int snk, float sc2, float lg, float2& dD, float2& r1, float2& r2,
                                         float2& r3) {
   const float2 m = make_float2(sc2, sc2), nl = make_float2(-lg, -lg);
 #pragma unroll
   for (int i = 0; i < CW; i += 2) {
     float2 s = __ffma2_rn(f2(vs[i], vs[i + 1]), m, nl);
     if (MASK) {
-      if (kc + i > khi || kc + i < klo) s.x = -INFINITY;
-      if (kc + i + 1 > khi || kc + i + 1 < klo) s.y = -INFINITY;
+      if (kc + i > khi || (kc + i < klo && (MASK == 1 || kc + i >= snk))) s.x = -INFINITY;
+      if (kc + i + 1 > khi || (kc + i + 1 < klo && (MASK == 1 || kc + i + 1 >= snk))) s.y = -INFINITY;
     }
     const float2 p = make_float2(ex2(s.x), ex2(s.y));
     const float2 dp = f2(vdp[i], vdp[i + 1]);
@@ -120,10 +123,10 @@ __device__ __forceinline__ void q_stats(const uint32_t (&vs)[CW], const uint32_t
 //   ddP = P u,  dS/scale = P (dP - D),
 //   dS2/scale = P (dPa + dP u - ddS D - B) = P (dPa - c) + ddP (dP - D).
 // Column pairs go through the packed fp32x2 instructions, as in q_stats.
-template <int CW, bool MASK>
+template <int CW, int MASK>
 __device__ __forceinline__ void q_ops(const uint32_t (&vs)[CW], const uint32_t (&vdds)[CW],
                                       const uint32_t (&vdp)[CW], const uint32_t (&vdpa)[CW], int kc, int klo, int khi,
-                                      float sc, float sc2, float lg, float dv, float dD, float cq,
+                                      int snk, float sc, float sc2, float lg, float dv, float dD, float cq,
                                       uint32_t (&o_ds)[CW / 2], uint32_t (&o_ds2)[CW / 2], uint32_t (&o_ddp)[CW / 2],
                                       uint32_t (&o_p)[CW / 2]) {
   const float2 m = make_float2(sc2, sc2), nl = make_float2(-lg, -lg), msc = make_float2(sc, sc);
@@ -132,8 +135,8 @@ __device__ __forceinline__ void q_ops(const uint32_t (&vs)[CW], const uint32_t (
   for (int i = 0; i < CW; i += 2) {
     float2 s = __ffma2_rn(f2(vs[i], vs[i + 1]), m, nl);
     if (MASK) {
-      if (kc + i > khi || kc + i < klo) s.x = -INFINITY;
-      if (kc + i + 1 > khi || kc + i + 1 < klo) s.y = -INFINITY;
+      if (kc + i > khi || (kc + i < klo && (MASK == 1 || kc + i >= snk))) s.x = -INFINITY;
+      if (kc + i + 1 > khi || (kc + i + 1 < klo && (MASK == 1 || kc + i + 1 >= snk))) s.y = -INFINITY;
     }
     const float2 p = make_float2(ex2(s.x), ex2(s.y));
     const float2 u = __ffma2_rn(f2(vdds[i], vdds[i + 1]), msc, ndd);  // ddS - dD
@@ -150,24 +153,24 @@ __device__ __forceinline__ void q_ops(const uint32_t (&vs)[CW], const uint32_t (
 
 // Forward-tangent forms (dO = 0): the stats sweep needs only dD/scale += P ddS', and
 // the second sweep only P and ddP = P (ddS - dD).
-template <int CW, bool MASK>
+template <int CW, int MASK>
 __device__ __forceinline__ void q_stats_tj(const uint32_t (&vs)[CW], const uint32_t (&vdds)[CW], int kc, int klo,
-                                           int khi, float sc2, float lg, float2& dD) {
+                                           int khi, int snk, float sc2, float lg, float2& dD) {
   const float2 m = make_float2(sc2, sc2), nl = make_float2(-lg, -lg);
 #pragma unroll
   for (int i = 0; i < CW; i += 2) {
     float2 s = __ffma2_rn(f2(vs[i], vs[i + 1]), m, nl);
     if (MASK) {
-      if (kc + i > khi || kc + i < klo) s.x = -INFINITY;
-      if (kc + i + 1 > khi || kc + i + 1 < klo) s.y = -INFINITY;
+      if (kc + i > khi || (kc + i < klo && (MASK == 1 || kc + i >= snk))) s.x = -INFINITY;
+      if (kc + i + 1 > khi || (kc + i + 1 < klo && (MASK == 1 || kc + i + 1 >= snk))) s.y = -INFINITY;
     }
     dD = __fadd2_rn(dD, __fmul2_rn(f2(vdds[i], vdds[i + 1]), make_float2(ex2(s.x), ex2(s.y))));
   }
 }
 
-template <int CW, bool MASK>
+template <int CW, int MASK>
 __device__ __forceinline__ void q_ops_tj(const uint32_t (&vs)[CW], const uint32_t (&vdds)[CW], int kc, int klo,
-                                         int khi, float sc, float sc2, float lg, float dD,
+                                         int khi, int snk, float sc, float sc2, float lg, float dD,
                                          uint32_t (&o_ddp)[CW / 2], uint32_t (&o_p)[CW / 2]) {
   const float2 m = make_float2(sc2, sc2), nl = make_float2(-lg, -lg), msc = make_float2(sc, sc);
   const float2 ndd = make_float2(-dD, -dD);
@@ -175,8 +178,8 @@ __device__ __forceinline__ void q_ops_tj(const uint32_t (&vs)[CW], const uint32_
   for (int i = 0; i < CW; i += 2) {
     float2 s = __ffma2_rn(f2(vs[i], vs[i + 1]), m, nl);
     if (MASK) {
-      if (kc + i > khi || kc + i < klo) s.x = -INFINITY;
-      if (kc + i + 1 > khi || kc + i + 1 < klo) s.y = -INFINITY;
+      if (kc + i > khi || (kc + i < klo && (MASK == 1 || kc + i >= snk))) s.x = -INFINITY;
+      if (kc + i + 1 > khi || (kc + i + 1 < klo && (MASK == 1 || kc + i + 1 >= snk))) s.y = -INFINITY;
     }
     const float2 p = make_float2(ex2(s.x), ex2(s.y));
     const float2 ddp = __fmul2_rn(p, __ffma2_rn(f2(vdds[i], vdds[i + 1]), msc, ndd));
@@ -189,7 +192,8 @@ __device__ __forceinline__ void q_ops_tj(const uint32_t (&vs)[CW], const uint32_
 // D = B = 0, dS = dS2 = 0 and dQ' = 0, and the pass reduces to the jvp of the forward:
 // ddO = ddP V + P ddV = tO and dD = rowsum(P ddS) = tL. It skips the dO products, the
 // dQ' products and dO's tile: 8 of the 14 GEMM-equivalents per pair remain.
-template <int HD, bool VL, bool TJ, bool GRP>
+// SNK: a window with sinks (the key tiles are SinkTiles).
+template <int HD, bool VL, bool TJ, bool GRP, bool SNK>
 __global__ void __launch_bounds__(kBBThreads, 1)
     bwdbwd_q_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                     const __grid_constant__ CUtensorMap tm_ddq, const __grid_constant__ CUtensorMap tm_k,
@@ -231,7 +235,15 @@ __global__ void __launch_bounds__(kBBThreads, 1)
   const AttnShape sh = seq_shape<VL>(a.sh, b, &sr);  // this sequence's lengths and mask; sr: where its rows start
   const int q0 = qt * kBM;
   int j0;
-  const int n = key_tiles(sh, q0, kBM, BN, &j0);  // key tiles j0, j0 + 1, ... per sweep (0: no row sees a key)
+  int n = 0;  // key tiles per sweep: j0, j0 + 1, ... or, with sinks, sink.tile(0), ... (0: no row sees a key)
+  SinkTiles sink{0, 0, 0};
+  if constexpr (SNK) {
+    sink = sink_key_tiles(sh, q0, kBM, BN);
+    n = sink.n;
+  } else {
+    n = key_tiles(sh, q0, kBM, BN, &j0);
+  }
+  auto key_row = [&](int it) { return (SNK ? sink.tile(it) : j0 + it) * BN; };  // first key of tile `it` of a sweep
   const int total = 2 * n;
   // Score buffer of tile `it` and how many earlier tiles used that buffer:
   // the stats sweep alternates buffers 0 and 1, the second sweep uses buffer 0.
@@ -284,7 +296,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
           raise_error(a.status, &abort_flag, kDevTimeoutSlotEmpty);
           break;
         }
-        const int k0 = (j0 + it % n) * BN;
+        const int k0 = key_row(it % n);
         uint8_t* slot = s_ring + s * G::SLOT;
         mbar_arrive_expect_tx(&bar_full[s], G::SLOT);
         tma_pair<HD>(slot, &tm_k, &tm_ddk, &bar_full[s], sr.k0 + k0, BN, h / sh.G, sr.bc);
@@ -441,20 +453,20 @@ __global__ void __launch_bounds__(kBBThreads, 1)
     if (ok && n > 0) {
       float2 pdD = make_float2(0.f, 0.f), pr1 = pdD, pr2 = pdD, pr3 = pdD;  // (even, odd) column partial sums
       for (int j = 0; ok && j < n; ++j) {
-        const int kc = (j0 + j) * BN + cb;  // first key of this thread's columns
+        const int kc = key_row(j) + cb;  // first key of this thread's columns
         uint32_t vs[CW], vdds[CW], vdp[CW], vdpa[CW];
         ok = load_scores(j, vs, vdds, vdp, vdpa);
         if (!ok) break;
         if constexpr (TJ) {
-          if (kc + CW - 1 > khi || kc < klo)
-            q_stats_tj<CW, true>(vs, vdds, kc, klo, khi, sc2, lg, pdD);
+          if (kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sh.sinks)))
+            q_stats_tj<CW, SNK ? 2 : 1>(vs, vdds, kc, klo, khi, sh.sinks, sc2, lg, pdD);
           else
-            q_stats_tj<CW, false>(vs, vdds, kc, klo, khi, sc2, lg, pdD);
+            q_stats_tj<CW, 0>(vs, vdds, kc, klo, khi, 0, sc2, lg, pdD);
         } else {
-          if (kc + CW - 1 > khi || kc < klo)
-            q_stats<CW, true>(vs, vdds, vdp, vdpa, kc, klo, khi, sc2, lg, pdD, pr1, pr2, pr3);
+          if (kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sh.sinks)))
+            q_stats<CW, SNK ? 2 : 1>(vs, vdds, vdp, vdpa, kc, klo, khi, sh.sinks, sc2, lg, pdD, pr1, pr2, pr3);
           else
-            q_stats<CW, false>(vs, vdds, vdp, vdpa, kc, klo, khi, sc2, lg, pdD, pr1, pr2, pr3);
+            q_stats<CW, 0>(vs, vdds, vdp, vdpa, kc, klo, khi, 0, sc2, lg, pdD, pr1, pr2, pr3);
         }
       }
       if (ok) {
@@ -478,21 +490,21 @@ __global__ void __launch_bounds__(kBBThreads, 1)
     }
     // Sweep 2: the bf16 operands of the accumulating MMAs.
     for (int j = 0; ok && j < n; ++j) {
-      const int kc = (j0 + j) * BN + cb;
+      const int kc = key_row(j) + cb;
       uint32_t vs[CW], vdds[CW], vdp[CW], vdpa[CW];
       ok = load_scores(n + j, vs, vdds, vdp, vdpa);
       if (!ok) break;
       uint32_t o_ds[CW / 2], o_ds2[CW / 2], o_ddp[CW / 2], o_p[CW / 2];
       if constexpr (TJ) {
-        if (kc + CW - 1 > khi || kc < klo)
-          q_ops_tj<CW, true>(vs, vdds, kc, klo, khi, sc, sc2, lg, dD, o_ddp, o_p);
+        if (kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sh.sinks)))
+          q_ops_tj<CW, SNK ? 2 : 1>(vs, vdds, kc, klo, khi, sh.sinks, sc, sc2, lg, dD, o_ddp, o_p);
         else
-          q_ops_tj<CW, false>(vs, vdds, kc, klo, khi, sc, sc2, lg, dD, o_ddp, o_p);
+          q_ops_tj<CW, 0>(vs, vdds, kc, klo, khi, 0, sc, sc2, lg, dD, o_ddp, o_p);
       } else {
-        if (kc + CW - 1 > khi || kc < klo)
-          q_ops<CW, true>(vs, vdds, vdp, vdpa, kc, klo, khi, sc, sc2, lg, dv, dD, cq, o_ds, o_ds2, o_ddp, o_p);
+        if (kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sh.sinks)))
+          q_ops<CW, SNK ? 2 : 1>(vs, vdds, vdp, vdpa, kc, klo, khi, sh.sinks, sc, sc2, lg, dv, dD, cq, o_ds, o_ds2, o_ddp, o_p);
         else
-          q_ops<CW, false>(vs, vdds, vdp, vdpa, kc, klo, khi, sc, sc2, lg, dv, dD, cq, o_ds, o_ds2, o_ddp, o_p);
+          q_ops<CW, 0>(vs, vdds, vdp, vdpa, kc, klo, khi, 0, sc, sc2, lg, dv, dD, cq, o_ds, o_ds2, o_ddp, o_p);
       }
       if (j > 0) ok = mbar_wait_warp(&bar_ops_empty, (j - 1) & 1, &abort_flag);
       if (!ok) break;
@@ -1010,16 +1022,6 @@ int launch_bwdbwd_hd(const AttnShape& s, const BwdBwdPtrs& p, int passes, int* s
        make_seq_map(&mk[5], p.dO ? p.dO : p.q, HD, s.total_q, s.H, map_batch(s), s.sq, GK::BN) &&
        make_seq_map(&mk[6], p.ddq, HD, s.total_q, s.H, map_batch(s), s.sq, GK::BN);
   if (!ok) return kInvalidArgument;
-  if (ensure_smem_limit(reinterpret_cast<const void*>(&bwdbwd_q_kernel<HD, VL, false, false>), GQ::SMEM) != kOk ||
-      ensure_smem_limit(reinterpret_cast<const void*>(&bwdbwd_q_kernel<HD, VL, true, false>), GQ::SMEM) != kOk ||
-      ensure_smem_limit(reinterpret_cast<const void*>(&bwdbwd_k_kernel<HD, VL, false>), GK::SMEM) != kOk)
-    return kLaunchFailed;
-  if constexpr (!VL) {
-    if (ensure_smem_limit(reinterpret_cast<const void*>(&bwdbwd_q_kernel<HD, false, false, true>), GQ::SMEM) != kOk ||
-        ensure_smem_limit(reinterpret_cast<const void*>(&bwdbwd_q_kernel<HD, false, true, true>), GQ::SMEM) != kOk ||
-        ensure_smem_limit(reinterpret_cast<const void*>(&bwdbwd_k_kernel<HD, false, true>), GK::SMEM) != kOk)
-      return kLaunchFailed;
-  }
   // With `o`, the query pass computes D into delta_out and the key pass reads it there.
   BBArgs args{s,
               p.lse,
@@ -1042,36 +1044,48 @@ int launch_bwdbwd_hd(const AttnShape& s, const BwdBwdPtrs& p, int passes, int* s
   // causal mask): its static snake balances work only over a heaviest-first sequence,
   // which a grouped causal order is not (measured: key pass 2.24 -> 3.00 ms at causal
   // B1 H32 S8192 D128), while the query pass is balanced by the block scheduler.
-  const bool grp_q = !VL && args.grp_q < s.H * s.B, grp_k = !VL && !s.causal && args.grp_k < s.Hk * s.B;
+  // With sinks the query tiles of a head share few of their keys: plain order.
+  const bool grp_q = !VL && s.sinks == 0 && args.grp_q < s.H * s.B;
+  const bool grp_k = !VL && !s.causal && args.grp_k < s.Hk * s.B;
   const int nq = (s.Tq + kBM - 1) / kBM;
   const dim3 gq(s.H, s.B, nq), gq_grouped(s.H * s.B * nq);
+  auto launch_q = [&](auto* kernel, dim3 grid) {
+    if (ensure_smem_limit(reinterpret_cast<const void*>(kernel), GQ::SMEM) != kOk) return kLaunchFailed;
+    kernel<<<grid, kBBThreads, GQ::SMEM, stream>>>(mq[0], mq[1], mq[2], mq[3], mq[4], mq[5], mq[6], mq[7], args);
+    return static_cast<HostStatus>(after_launch());
+  };
+  auto launch_k = [&](auto* kernel, dim3 grid) {
+    if (ensure_smem_limit(reinterpret_cast<const void*>(kernel), GK::SMEM) != kOk) return kLaunchFailed;
+    kernel<<<grid, kBBThreads, GK::SMEM, stream>>>(mk[0], mk[1], mk[2], mk[3], mk[4], mk[5], mk[6], args);
+    return static_cast<HostStatus>(after_launch());
+  };
   if (passes & (kPassFwdTangent | kPassQuery)) {
     const bool tj = (passes & kPassFwdTangent) != 0;
-#define FH_Q_LAUNCH(TJ_, GRP_, GRID)                                                                       \
-  bwdbwd_q_kernel<HD, GRP_ ? false : VL, TJ_, GRP_><<<GRID, kBBThreads, GQ::SMEM, stream>>>(                 \
-      mq[0], mq[1], mq[2], mq[3], mq[4], mq[5], mq[6], mq[7], args)
-    if (grp_q) {
-      if (tj) FH_Q_LAUNCH(true, true, gq_grouped);
-      else FH_Q_LAUNCH(false, true, gq_grouped);
-    } else if (tj) {
-      FH_Q_LAUNCH(true, false, gq);
-    } else {
-      FH_Q_LAUNCH(false, false, gq);
+    HostStatus rc = kOk;
+    bool done = false;
+    if constexpr (!VL) {
+      if (grp_q) {
+        rc = tj ? launch_q(&bwdbwd_q_kernel<HD, false, true, true, false>, gq_grouped)
+                : launch_q(&bwdbwd_q_kernel<HD, false, false, true, false>, gq_grouped);
+        done = true;
+      }
     }
-#undef FH_Q_LAUNCH
-    if (after_launch() != kOk) return kLaunchFailed;
+    if (!done && s.sinks > 0)
+      rc = tj ? launch_q(&bwdbwd_q_kernel<HD, VL, true, false, true>, gq)
+              : launch_q(&bwdbwd_q_kernel<HD, VL, false, false, true>, gq);
+    else if (!done)
+      rc = tj ? launch_q(&bwdbwd_q_kernel<HD, VL, true, false, false>, gq)
+              : launch_q(&bwdbwd_q_kernel<HD, VL, false, false, false>, gq);
+    if (rc != kOk) return rc;
   }
   if (passes & kPassKey) {
     // Persistent: one CTA per SM (at most one per work item).
     const int items = s.Hk * s.B * ((s.Tk + kBM - 1) / kBM);
     const dim3 gk(static_cast<unsigned>(items < sm_count() ? items : sm_count()));
-    if (grp_k)
-      bwdbwd_k_kernel<HD, false, true><<<gk, kBBThreads, GK::SMEM, stream>>>(mk[0], mk[1], mk[2], mk[3], mk[4], mk[5],
-                                                                             mk[6], args);
-    else
-      bwdbwd_k_kernel<HD, VL, false><<<gk, kBBThreads, GK::SMEM, stream>>>(mk[0], mk[1], mk[2], mk[3], mk[4], mk[5],
-                                                                            mk[6], args);
-    if (after_launch() != kOk) return kLaunchFailed;
+    if constexpr (!VL) {
+      if (grp_k) return launch_k(&bwdbwd_k_kernel<HD, false, true>, gk);
+    }
+    return launch_k(&bwdbwd_k_kernel<HD, VL, false>, gk);
   }
   return kOk;
 }

@@ -142,7 +142,10 @@ int validate(const fh_attn_dims* d, AttnShape* out, float scale, int causal, boo
   out->scale = scale;
   out->causal = causal ? 1 : 0;
   out->br = causal == 2 ? 1 : 0;
+  if (d->sinks < 0) return fail(kInvalidArgument, "sinks must be >= 0");
+  if (d->sinks > 0 && !d->window) return fail(kInvalidArgument, "sinks need a sliding window");
   out->window = d->window;
+  out->sinks = d->sinks;
   out->total_q = d->seq_q;
   out->total_k = d->seq_k;
   if (varlen) {
@@ -156,6 +159,7 @@ int validate(const fh_attn_dims* d, AttnShape* out, float scale, int causal, boo
   } else {
     out->cu_q = out->cu_k = nullptr;
     out->diag = causal == 2 ? d->seq_k - d->seq_q : 0;
+    if (d->seq_q + out->diag <= d->window) out->sinks = 0;  // the window hides nothing
   }
   return kOk;
 }

@@ -61,7 +61,7 @@ __device__ __forceinline__ float max16(float x) {
 }
 
 __device__ __forceinline__ bool visible(const AttnShape& s, int i, int j) {
-  return i < s.Tq && j < s.Tk && j >= key_lo(s, i) && j <= key_hi(s, i);
+  return i < s.Tq && j < s.Tk && j <= key_hi(s, i) && (j >= key_lo(s, i) || j < s.sinks);
 }
 
 // rows [row0, row0 + ROWS) of head h of batch b (zeros past `len`) into a
@@ -299,16 +299,16 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas<HD>)
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = -INFINITY, l[i] = 0.f;
   zero(acc);
-  int first;
-  const int nt = key_tiles(s, r0, kRes, G::BN, &first);
+  const SinkTiles tiles = sink_key_tiles(s, r0, kRes, G::BN);
+  const int nt = tiles.n;
   auto fetch = [&](int t) {
     float* buf = sKV + (t & 1) * 2 * G::STR;
-    load_rows_async<HD, G::BN>(buf, k, s.sk, b, hk, (first + t) * G::BN, s.Tk);
-    load_rows_async<HD, G::BN>(buf + G::STR, v, s.sk, b, hk, (first + t) * G::BN, s.Tk);
+    load_rows_async<HD, G::BN>(buf, k, s.sk, b, hk, tiles.tile(t) * G::BN, s.Tk);
+    load_rows_async<HD, G::BN>(buf + G::STR, v, s.sk, b, hk, tiles.tile(t) * G::BN, s.Tk);
   };
   if (nt > 0) fetch(0);
   for (int it = 0; it < nt; ++it) {
-    const int c0 = (first + it) * G::BN;
+    const int c0 = tiles.tile(it) * G::BN;
     // Buffer (it + 1) & 1 was last read in iteration it - 1, which ended with a barrier.
     if (it + 1 < nt) {
       fetch(it + 1);
@@ -410,10 +410,10 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas<HD>)
   }
   float acc[4][G::NO];
   zero(acc);
-  int first;
-  const int nt = key_tiles(s, r0, kRes, G::BN, &first);
+  const SinkTiles tiles = sink_key_tiles(s, r0, kRes, G::BN);
+  const int nt = tiles.n;
   for (int it = 0; it < nt; ++it) {
-    const int c0 = (first + it) * G::BN;
+    const int c0 = tiles.tile(it) * G::BN;
     __syncthreads();
     load_rows<HD, G::BN>(sK, k, s.sk, b, hk, c0, s.Tk);
     load_rows<HD, G::BN>(sV, v, s.sk, b, hk, c0, s.Tk);
@@ -537,15 +537,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     L[i] = row < s.Tq ? lse[stat_index(s, b, h, row)] : 0.f;
     D[i] = row < s.Tq ? delta[stat_index(s, b, h, row)] : 0.f;
   }
-  int first;
-  const int nt = key_tiles(s, r0, kRes, G::BN, &first);
+  const SinkTiles tiles = sink_key_tiles(s, r0, kRes, G::BN);
+  const int nt = tiles.n;
 
   // Items u = 0 .. 2 nt - 1: sweep 1 (row statistics) over the key tiles, then sweep 2
   // (dQ', ddO) over the same tiles. With two buffers, item u + 1's tile is fetched
   // (cp.async) while item u's is used, across the sweep boundary too.
   const int total = 2 * nt;
   auto fetch = [&](int u) {
-    const int c0 = (first + u % nt) * G::BN;
+    const int c0 = tiles.tile(u % nt) * G::BN;
     float* buf = kbuf + (u % NBUF) * BUF;
     load_rows_async<HD, G::BN>(buf, k, s.sk, b, hk, c0, s.Tk);
     load_rows_async<HD, G::BN>(buf + G::STR, v, s.sk, b, hk, c0, s.Tk);
@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (NBUF == 2 && total > 0) fetch(0);
   for (int u = 0; u < total; ++u) {
-    const int c0 = (first + u % nt) * G::BN;
+    const int c0 = tiles.tile(u % nt) * G::BN;
     if (NBUF == 2) {
       // Buffer (u + 1) % 2 was last read in item u - 1, which ended with a barrier.
       if (u + 1 < total) {

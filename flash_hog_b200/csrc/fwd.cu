@@ -112,7 +112,9 @@ __device__ __forceinline__ void fwd_warp_arrive(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-template <int HD, bool VL, bool GRP>
+// SNK: a window with sinks. The ring then streams the sinks' key tiles before the
+// window's (SinkTiles), and both query tiles of a CTA take all of them.
+template <int HD, bool VL, bool GRP, bool SNK>
 __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
     fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const FwdArgs a) {
@@ -149,8 +151,15 @@ __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
   // tile lies past the last query row or sees no key). The ring streams the
   // union [jlo, jlo + n); tile t joins at ring position at[t].
   int nt[2] = {0, 0}, jt[2] = {0, 0}, at[2] = {0, 0};
+  SinkTiles sink{0, 0, 0};
+  if constexpr (SNK) {
+    sink = sink_key_tiles(sh, q0, G::ROWS, BN);
 #pragma unroll
-  for (int t = 0; t < T; ++t) nt[t] = key_tiles(sh, q0 + t * kBM, kBM, BN, &jt[t]);
+    for (int t = 0; t < T; ++t) nt[t] = q0 + t * kBM < sh.Tq ? sink.n : 0;
+  } else {
+#pragma unroll
+    for (int t = 0; t < T; ++t) nt[t] = key_tiles(sh, q0 + t * kBM, kBM, BN, &jt[t]);
+  }
   const int jlo = nt[0] > 0 ? (nt[1] > 0 ? min(jt[0], jt[1]) : jt[0]) : jt[1];
   int jhi = jlo;
 #pragma unroll
@@ -159,6 +168,7 @@ __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
     at[t] = jt[t] - jlo;
   }
   const int n = jhi - jlo;  // key tiles streamed (0 if no row sees a key)
+  auto key_row = [&](int j) { return (SNK ? sink.tile(j) : jlo + j) * BN; };  // first key of ring position j
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -201,14 +211,14 @@ __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
           break;
         }
         mbar_arrive_expect_tx(&bar_kfull[s], G::STR);
-        tma_rows<HD>(slot, &tm_k, &bar_kfull[s], sr.k0 + (jlo + j) * BN, BN, h / sh.G, sr.bc);
+        tma_rows<HD>(slot, &tm_k, &bar_kfull[s], sr.k0 + key_row(j), BN, h / sh.G, sr.bc);
         k_issued = j + 1;
         if (j >= ST && !mbar_wait(&bar_vempty[s], ph, &abort_flag)) {
           raise_error(a.status, &abort_flag, kDevTimeoutSlotEmpty);
           break;
         }
         mbar_arrive_expect_tx(&bar_vfull[s], G::STR);
-        tma_rows<HD>(slot + G::STR, &tm_v, &bar_vfull[s], sr.k0 + (jlo + j) * BN, BN, h / sh.G, sr.bc);
+        tma_rows<HD>(slot + G::STR, &tm_v, &bar_vfull[s], sr.k0 + key_row(j), BN, h / sh.G, sr.bc);
         v_issued = j + 1;
       }
       // Every issued copy must land before this CTA's shared memory is released.
@@ -312,7 +322,7 @@ __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
     const int row = q0 + t * kBM + r;
     const bool row_ok = row < sh.Tq;
     int jt0;  // first key tile of this warpgroup's query tile
-    const int nj = key_tiles(sh, q0 + t * kBM, kBM, BN, &jt0);
+    const int nj = SNK ? nt[t] : key_tiles(sh, q0 + t * kBM, kBM, BN, &jt0);
     const int khi = key_hi(sh, row), klo = key_lo(sh, row);  // this row's visible keys
     const float sc2 = sh.scale * kLog2e;
     const uint32_t lane_base = tmem + tmem_lane_base(warp & 3);
@@ -321,7 +331,7 @@ __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
     float m_used = -INFINITY, l = 0.f;  // running maximum (log2 domain) and the sum against it
     bool ok = true;
     for (int j = 0; j < nj; ++j) {
-      const int k0 = (jt0 + j) * BN;
+      const int k0 = SNK ? key_row(j) : (jt0 + j) * BN;
       ok = mbar_wait_warp(&bar_s_full[t], j & 1, &abort_flag);
       if (!ok) break;
       tc_fence_after();
@@ -332,10 +342,10 @@ __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
 #pragma unroll
       for (int i = 0; i < BN; ++i) asm volatile("" : "+r"(v[i])::"memory");
       if constexpr (G::SEP_P) fwd_warp_arrive(&bar_s_empty[t]);  // S(j+1) may be computed now
-      if (k0 + BN - 1 > khi || k0 < klo) {
+      if (k0 + BN - 1 > khi || (k0 < klo && (!SNK || k0 + BN > sh.sinks))) {
 #pragma unroll
         for (int i = 0; i < BN; ++i)
-          if (k0 + i > khi || k0 + i < klo) v[i] = __float_as_uint(-INFINITY);
+          if (k0 + i > khi || (k0 + i < klo && (!SNK || k0 + i >= sh.sinks))) v[i] = __float_as_uint(-INFINITY);
       }
       // Row maximum of the raw scores (the scale is positive), eight independent chains.
       float mx[8];
@@ -444,20 +454,22 @@ int launch_fwd_hd(const AttnShape& s, const FwdPtrs& p, int* status, cudaStream_
       !make_seq_map(&mk, p.k, HD, s.total_k, s.Hk, map_batch(s), s.sk, G::BN) ||
       !make_seq_map(&mv, p.v, HD, s.total_k, s.Hk, map_batch(s), s.sk, G::BN))
     return kInvalidArgument;
-  if (ensure_smem_limit(reinterpret_cast<const void*>(&fwd_kernel<HD, VL, false>), G::SMEM) != kOk) return kLaunchFailed;
-  if constexpr (!VL) {
-    if (ensure_smem_limit(reinterpret_cast<const void*>(&fwd_kernel<HD, false, true>), G::SMEM) != kOk)
-      return kLaunchFailed;
-  }
   // K and V of a key head are the tiles the query tiles of its heads share.
   FwdArgs args{s, static_cast<__nv_bfloat16*>(p.o), p.lse, status,
                locality_group(s.H * s.B, s.H / s.Hk, 2ll * s.Tk * HD * 2)};
   const int nq = (s.Tq + G::ROWS - 1) / G::ROWS;
-  if (!VL && args.grp < s.H * s.B)  // grouped only where the groups split the pairs
-    fwd_kernel<HD, false, true><<<dim3(s.H * s.B * nq), G::THREADS, G::SMEM, stream>>>(mq, mk, mv, args);
-  else
-    fwd_kernel<HD, VL, false><<<dim3(s.H, s.B, nq), G::THREADS, G::SMEM, stream>>>(mq, mk, mv, args);
-  return after_launch();
+  auto launch = [&](auto* kernel, dim3 grid) {
+    if (ensure_smem_limit(reinterpret_cast<const void*>(kernel), G::SMEM) != kOk) return kLaunchFailed;
+    kernel<<<grid, G::THREADS, G::SMEM, stream>>>(mq, mk, mv, args);
+    return static_cast<HostStatus>(after_launch());
+  };
+  const dim3 grid(s.H, s.B, nq);
+  // Sinks: a query tile shares few of its keys with the head's other tiles, plain order.
+  if (s.sinks > 0) return launch(&fwd_kernel<HD, VL, false, true>, grid);
+  if constexpr (!VL) {  // grouped only where the groups split the pairs
+    if (args.grp < s.H * s.B) return launch(&fwd_kernel<HD, false, true, false>, dim3(s.H * s.B * nq));
+  }
+  return launch(&fwd_kernel<HD, VL, false, false>, grid);
 }
 
 }  // namespace

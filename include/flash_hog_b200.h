@@ -110,6 +110,9 @@ typedef struct fh_attn_dims {
   const int32_t* cu_seqlens_k;
   int32_t max_seqlen_q;
   int32_t max_seqlen_k;
+  /* First keys that stay visible behind a sliding window (0 = none; needs window > 0):
+   * query i also sees keys j < sinks with j <= diag_i. Per sequence in a packed batch. */
+  int32_t sinks;
 } fh_attn_dims;
 
 /* Forward: o = softmax(scale * q k^T + mask) v, lse = logsumexp(scale * q k^T + mask).

@@ -49,18 +49,20 @@ def default_scale(head_dim: int) -> float:
     return head_dim ** -0.5
 
 
-def causal_mask(nq: int, nk: int, causal=1, window: int = 0) -> np.ndarray:
+def causal_mask(nq: int, nk: int, causal=1, window=0) -> np.ndarray:
     """Causal band mask, True where the score is kept: query i sees key j iff
     j <= i + diag and (window == 0 or i + diag - j < window), with diag = 0 for
     ``causal`` 1 / True (top-left, ``_pallas_gpu_kernel.py:37-41``) and nk - nq for
     ``causal`` 2 (bottom-right: ``get_mask_bottom_right``'s ``qi = qi + ks - qs``,
     ``(qi >= kj) & (qi - kj < sliding_window_length)``,
-    ``flash_hog/_jax_refs/jax_impl.py:104-109``)."""
+    ``flash_hog/_jax_refs/jax_impl.py:104-109``). A ``window`` (length, sinks) keeps the
+    first ``sinks`` keys visible behind it."""
+    window, sinks = window if isinstance(window, tuple) else (window, 0)
     qi = np.arange(nq)[:, None] + (nk - nq if int(causal) == 2 else 0)
     kj = np.arange(nk)[None, :]
     keep = qi >= kj
     if window:
-        keep &= (qi - kj) < window
+        keep &= ((qi - kj) < window) | (kj < sinks)
     return keep
 
 
