@@ -129,7 +129,9 @@ def _is_f32(x: torch.Tensor, policy: str | None = None, mask=None) -> bool:
 
 def _operand(x: torch.Tensor, f32: bool) -> torch.Tensor:
     """BTNH with a contiguous layout in the kernels' operand type (fp32 or bf16)."""
-    x = x.to(torch.float32 if f32 else torch.bfloat16)
+    dtype = torch.float32 if f32 else torch.bfloat16
+    if x.dtype is not dtype:
+        x = x.to(dtype)
     return x if x.is_contiguous() else x.contiguous()
 
 
@@ -176,7 +178,8 @@ def cuda_dot_product_attention(query, key, value, mask_type: MaskType, scale: fl
         _capi.attn_fwd_f32(q, k, v, out, lse, scale, *_mask_args(mask_type), **_mask_kw(mask_type))
     else:
         _capi.attn_fwd(q, k, v, out, lse, scale, *_mask_args(mask_type), **_mask_kw(mask_type))
-    out = out.to(query.dtype)
+    if out.dtype is not query.dtype:
+        out = out.to(query.dtype)
     return (out, lse) if return_residual else out
 
 

@@ -264,12 +264,14 @@ def make_dims(q: torch.Tensor, k: torch.Tensor, window: int = 0, varlen: Varlen 
 def _same_layout(ref: torch.Tensor, *others: torch.Tensor, dtype=torch.bfloat16) -> None:
     """Checks shape, strides, dtype and device against ``ref`` (None entries,
     unused outputs, are skipped)."""
+    shape, stride, device = ref.shape, ref.stride(), ref.device
     for t in (ref,) + others:
         if t is None:
             continue
-        if _layout_key(t) != _layout_key(ref):
+        # Equal strides at once; otherwise by the layout alone (size-1 dimensions aside).
+        if t.shape != shape or (t.stride() != stride and _layout_key(t) != _layout_key(ref)):
             raise ValueError("tensors of one side must share shape and strides")
-        if t.dtype != dtype or t.device != ref.device:
+        if t.dtype is not dtype or t.device != device:
             raise ValueError(f"tensors must be {dtype} on the same CUDA device")
 
 

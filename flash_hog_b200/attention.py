@@ -31,7 +31,10 @@ kernels run once, the rule the reference gives its double backward
 
 from __future__ import annotations
 
+import inspect
+
 import torch
+from torch.autograd import forward_ad
 
 from flash_hog_b200 import _attention_impl as attn_impl
 from flash_hog_b200._attention_impl import MaskType, PackedSequences, SlidingWindow
@@ -80,7 +83,12 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
         query, key, value = query.unsqueeze(0), key.unsqueeze(0), value.unsqueeze(0)
     # The fp32 policy is decided once here and kept with the residuals: the backward,
     # double backward and forward-mode rules of this graph all follow it.
-    result, _ = _DotProductAttention.apply(query, key, value, mask_type, float(scale), attn_impl.fp32_policy())
+    policy = attn_impl.fp32_policy()
+    if _untracked(query, key, value):
+        result = attn_impl.cuda_dot_product_attention(query, key, value, mask_type=mask_type, scale=float(scale),
+                                                      policy=policy)
+    else:
+        result, _ = _DotProductAttention.apply(query, key, value, mask_type, float(scale), policy)
     if unbatched:
         result = result.squeeze(0)
     return result
@@ -120,6 +128,22 @@ def _no_packed_vmap(mask_type):
         raise NotImplementedError("packed variable-length batches are not vmapped: pack the sequences instead")
 
 
+def _untracked(*ts) -> bool:
+    """Whether no derivative of a call on ``ts`` will be asked for, and no transform is at
+    work on them: the kernel is called without an autograd node (about 20 us of host time)."""
+    if forward_ad._current_level >= 0 or any(torch._C._functorch.is_functorch_wrapped_tensor(t) for t in ts):
+        return False
+    return not torch.is_grad_enabled() or not any(t.requires_grad for t in ts)
+
+
+def _plain_backward(g) -> bool:
+    """Whether a backward runs for its values alone: no graph of it is being built, and no
+    forward-mode or ``torch.func`` transform is differentiating or batching it. It then
+    calls the rule itself instead of an autograd node (about 30 us of host time less)."""
+    return (not torch.is_grad_enabled() and forward_ad._current_level < 0
+            and not torch._C._functorch.is_functorch_wrapped_tensor(g))
+
+
 class _DotProductAttention(torch.autograd.Function):
     """Forward (outputs O and the log-sum-exp L, the latter non-differentiable)."""
 
@@ -133,15 +157,25 @@ class _DotProductAttention(torch.autograd.Function):
         query, key, value, mask_type, scale, policy = inputs
         out, activation = output
         ctx.mark_non_differentiable(activation)
+        # A second backward reaches this node with no cotangent of `out` (the double
+        # backward's formulas carry that path): None instead of zeros spares a pass on them.
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(query, key, value, activation, out)
         ctx.save_for_forward(query, key, value, activation, out)
         ctx.mask_type, ctx.scale, ctx.policy = mask_type, scale, policy
 
     @staticmethod
     def backward(ctx, g, _g_activation):
+        if g is None:
+            return None, None, None, None, None, None
         query, key, value, activation, out = ctx.saved_tensors
-        dq, dk, dv = _DotProductAttentionBwd.apply(query, key, value, activation, out, g, ctx.mask_type, ctx.scale,
-                                                   ctx.policy)
+        if _plain_backward(g):
+            dq, dk, dv = attn_impl.dot_product_attention_bwd_rule(
+                mask_type=ctx.mask_type, scale=ctx.scale, res=(query, key, value, activation, out), g=g,
+                policy=ctx.policy)
+        else:
+            dq, dk, dv = _DotProductAttentionBwd.apply(query, key, value, activation, out, g, ctx.mask_type, ctx.scale,
+                                                       ctx.policy)
         return dq, dk, dv, None, None, None
 
     @staticmethod
@@ -174,6 +208,7 @@ class _DotProductAttentionBwd(torch.autograd.Function):
     @staticmethod
     def setup_context(ctx, inputs, output):
         query, key, value, activation, out, g, mask_type, scale, policy = inputs
+        ctx.set_materialize_grads(False)
         # The residual order of the reference's bwd-of-bwd rule (_attention_impl.py:264-275).
         ctx.save_for_backward(query, key, value, out, activation, g)
         ctx.save_for_forward(query, key, value, activation, out, g)
@@ -200,3 +235,9 @@ class _DotProductAttentionBwd(torch.autograd.Function):
         args = [attn_impl._fold(x, d, size) for x, d in zip((query, key, value, activation, out, g), in_dims[:6])]
         dq, dk, dv = _DotProductAttentionBwd.apply(*args, mask_type, scale, policy)
         return tuple(attn_impl._unfold(x, size) for x in (dq, dk, dv)), (0, 0, 0)
+
+
+# torch binds the arguments of a Function with setup_context to forward's signature in
+# every call; kept on the function, it is not worked out again each time (25 us).
+for _f in (_DotProductAttention, _DotProductAttentionBwd):
+    _f.forward.__signature__ = inspect.signature(_f.forward)

@@ -17,6 +17,7 @@ GPU generation: every call runs the sm_100a kernels or raises.
 from __future__ import annotations
 
 import dataclasses
+import inspect
 
 import torch
 
@@ -126,3 +127,6 @@ class _FlashBwdBwd(torch.autograd.Function):
         stats = stats.reshape(3, size, stats.shape[1] // size, *stats.shape[2:])
         return (_unfold(dq2, size), _unfold(dk2, size), _unfold(dv2, size), _unfold(ddo, size), stats), (0, 0, 0, 0, 1)
 
+
+# As for the Functions of attention.py: the signature is worked out once.
+_FlashBwdBwd.forward.__signature__ = inspect.signature(_FlashBwdBwd.forward)
