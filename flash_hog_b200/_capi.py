@@ -32,6 +32,7 @@ STATUS_NAMES = {
 
 # Every symbol include/flash_hog_b200.h declares.
 EXPORTED_SYMBOLS = (
+    "fh_attn_sink_scratch_floats",
     "fh_attn_fwd",
     "fh_attn_rowdot",
     "fh_attn_bwd",
@@ -98,6 +99,7 @@ class FhAttnDims(ctypes.Structure):
         ("max_seqlen_q", ctypes.c_int32),
         ("max_seqlen_k", ctypes.c_int32),
         ("sinks", ctypes.c_int32),
+        ("sink_scratch", ctypes.c_void_p),
     ]
 
 
@@ -114,6 +116,8 @@ def lib() -> ctypes.CDLL:
     h = ctypes.CDLL(path)
     vp, i32, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
     dims = ctypes.POINTER(FhAttnDims)
+    h.fh_attn_sink_scratch_floats.argtypes = [dims, i32]
+    h.fh_attn_sink_scratch_floats.restype = ctypes.c_longlong
     h.fh_attn_fwd.argtypes = [vp, dims, vp, vp, vp, vp, vp, f32, i32]
     h.fh_attn_rowdot.argtypes = [vp, dims, vp, vp, vp]
     h.fh_attn_bwd.argtypes = [vp, dims, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, f32, i32]
@@ -261,6 +265,18 @@ def make_dims(q: torch.Tensor, k: torch.Tensor, window: int = 0, varlen: Varlen 
     return dims
 
 
+def _sink_scratch(dims: FhAttnDims, causal: int, device):
+    """Sets the scratch of a backward with sinks in ``dims``; the result keeps it alive."""
+    if dims.sinks == 0:
+        return None
+    n = int(lib().fh_attn_sink_scratch_floats(ctypes.byref(dims), int(causal)))
+    if n <= 0:  # not used, or dims that the call itself will refuse
+        return None
+    scratch = torch.empty(n, dtype=torch.float32, device=device)
+    dims.sink_scratch = scratch.data_ptr()
+    return scratch
+
+
 def _same_layout(ref: torch.Tensor, *others: torch.Tensor, dtype=torch.bfloat16) -> None:
     """Checks shape, strides, dtype and device against ``ref`` (None entries,
     unused outputs, are skipped)."""
@@ -294,11 +310,12 @@ def attn_rowdot(o, dO, delta, varlen: Varlen | None = None) -> None:
 
 
 @_on_device
-def attn_bwd(q, k, v, o, dO, lse, dq, dk, dv, delta, scale: float, causal: int, window: int = 0, varlen: Varlen | None = None,
-             sinks: int = 0) -> None:
+def attn_bwd(q, k, v, o, dO, lse, dq, dk, dv, delta, scale: float, causal: int, window: int = 0,
+             varlen: Varlen | None = None, sinks: int = 0) -> None:
     _same_layout(q, o, dO, dq)
     _same_layout(k, v, dk, dv)
     dims = make_dims(q, k, window, varlen, sinks)
+    scratch = _sink_scratch(dims, causal, q.device)  # noqa: F841 - held until the call is queued
     _check("fh_attn_bwd", lib().fh_attn_bwd(_stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v),
                                            _ptr(o), _ptr(dO), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv),
                                            _ptr(delta), float(scale), int(causal)))
@@ -311,6 +328,7 @@ def attn_bwdbwd(q, k, v, dO, ddq, ddk, ddv, lse, delta, dq2, ddo, dk2, dv2, dd, 
     _same_layout(q, dO, ddq, dq2, ddo)
     _same_layout(k, v, ddk, ddv, dk2, dv2)
     dims = make_dims(q, k, window, varlen, sinks)
+    scratch = _sink_scratch(dims, causal, q.device)  # noqa: F841 - held until the call is queued
     _check("fh_attn_bwdbwd", lib().fh_attn_bwdbwd(
         _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(dO), _ptr(ddq), _ptr(ddk),
         _ptr(ddv), _ptr(lse), _ptr(delta), _ptr(dq2), _ptr(ddo), _ptr(dk2), _ptr(dv2), _ptr(dd), _ptr(bvec),
@@ -328,6 +346,7 @@ def attn_bwdbwd_pass(q, k, v, dO, ddq, ddk, ddv, lse, delta, dq2, ddo, dk2, dv2,
     _same_layout(q, dO, ddq, dq2, ddo)
     _same_layout(k, v, ddk, ddv, dk2, dv2)
     dims = make_dims(q, k, window, varlen, sinks)
+    scratch = _sink_scratch(dims, causal, q.device)  # noqa: F841 - held until the call is queued
     _check("fh_attn_bwdbwd_pass", lib().fh_attn_bwdbwd_pass(
         _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(dO), _ptr(ddq), _ptr(ddk),
         _ptr(ddv), _ptr(lse), _ptr(delta), _ptr(dq2), _ptr(ddo), _ptr(dk2), _ptr(dv2), _ptr(dd), _ptr(bvec),
@@ -342,6 +361,7 @@ def attn_bwdbwd_o(q, k, v, o, dO, ddq, ddk, ddv, lse, dq2, ddo, dk2, dv2, delta,
     _same_layout(q, o, dO, ddq, dq2, ddo)
     _same_layout(k, v, ddk, ddv, dk2, dv2)
     dims = make_dims(q, k, window, varlen, sinks)
+    scratch = _sink_scratch(dims, causal, q.device)  # noqa: F841 - held until the call is queued
     _check("fh_attn_bwdbwd_o", lib().fh_attn_bwdbwd_o(
         _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dO), _ptr(ddq),
         _ptr(ddk), _ptr(ddv), _ptr(lse), _ptr(dq2), _ptr(ddo), _ptr(dk2), _ptr(dv2), _ptr(delta), _ptr(dd),
@@ -356,6 +376,7 @@ def attn_jvp_bwd(q, k, v, o, dO, lse, tq, tk, tv, tdO, tdq, tdk, tdv, to, delta,
     _same_layout(q, o, dO, tq, tdq, to, tdO)
     _same_layout(k, v, tk, tv, tdk, tdv)
     dims = make_dims(q, k, window, varlen, sinks)
+    scratch = _sink_scratch(dims, causal, q.device)  # noqa: F841 - held until the call is queued
     _check("fh_attn_jvp_bwd", lib().fh_attn_jvp_bwd(
         _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dO), _ptr(lse), _ptr(tq),
         _ptr(tk), _ptr(tv), _ptr(tdO), _ptr(tdq), _ptr(tdk), _ptr(tdv), _ptr(to),

@@ -65,6 +65,8 @@ struct AttnShape {
   const int* cu_k;
   int total_q, total_k;       // rows of the packed tensors (varlen); Tq, Tk (dense)
   int sinks;                  // first keys that a window leaves visible (0 without a window)
+  int splits;                 // parts the key passes cut a sink tile's queries into (sink_splits)
+  float* sink_part;           // splits > 1: their fp32 partial sums (sink_part_floats)
 };
 
 // Where sequence b's rows start: the batch coordinate of its tensors' views and
@@ -182,6 +184,66 @@ inline int locality_group(int pairs, int shared, long long bytes_per_head) {
   long long g = kGroupBytes / (bytes_per_head > 0 ? bytes_per_head : 1);
   g = (g < 1 ? 1 : g) * shared;
   return g < pairs ? static_cast<int>(g) : pairs;
+}
+
+// Key tiles (of kBM keys) that hold a sink.
+__host__ __device__ __forceinline__ int sink_tiles(const AttnShape& s) {
+  return (min(s.sinks, s.Tk) + kBM - 1) / kBM;
+}
+
+// Parts into which the key passes cut the queries of a key tile that holds a sink: every
+// query sees it, where an ordinary tile is seen by about window + kBM of them, so a CTA
+// with a whole one may still run when the others are done (causal B1 H8 Hk2 S8000 D128,
+// window 2048: dK/dV 476 us whole, 128 us in 4 parts and the join 3 us). As many parts as
+// make them about equal to ordinary tiles, but no more than it takes to fill the GPU a few
+// times over: each costs a partial sum of 2 x kBM x head_dim floats and a share of the join.
+inline int sink_splits(const AttnShape& s) {
+  const long long own = static_cast<long long>(s.window) + kBM + 64;
+  if (s.sinks <= 0 || own >= s.Tq) return 1;
+  const long long parts = (s.Tq + own - 1) / own;
+  const long long most = 4 * 148 / (static_cast<long long>(s.Hk) * s.B * sink_tiles(s));
+  return static_cast<int>(parts < most ? parts : most < 1 ? 1 : most);
+}
+// Whether a kernel whose CTAs the block scheduler balances does better with whole sink
+// tiles: they start first and the others run beside them, so they may take 3/4 of an SM's
+// share of the work (dK/dV at B4 H16 S2048 D64, window 512: 80 us whole, 90 us in 3 parts
+// with the join). The persistent key pass of the double backward deals its items out in
+// advance and wants equal ones (B4 H12 S1024 D64, window 256: 48 us
+// whole, 45 us in parts with the join; 120 and 119 us at the shape above).
+inline bool sink_whole(const AttnShape& s) {
+  const long long own = static_cast<long long>(s.window) + kBM + 64;
+  const long long ns = sink_tiles(s), nk = (s.Tk + kBM - 1) / kBM;
+  return 4ll * s.Tq <= 3 * (static_cast<long long>(s.Hk) * s.B * ((nk - ns) * own + ns * s.Tq) / 148);
+}
+inline long long sink_part_floats(const AttnShape& s, int hd, int splits) {
+  return splits > 1 ? 2ll * kBM * hd * splits * s.Hk * s.B * sink_tiles(s) : 0;
+}
+
+// Work of a key pass with split sink tiles, in slots of (key tile, part): first the parts
+// of the sink tiles, then the ordinary tiles whole.
+__host__ __device__ __forceinline__ int split_slots(const AttnShape& s, int tiles) {
+  return tiles + min(sink_tiles(s), tiles) * (s.splits - 1);
+}
+// Slot z's key tile; *part: which part of it, -1 = whole.
+__device__ __forceinline__ int split_slot(const AttnShape& s, int z, int* part) {
+  const int cut = sink_tiles(s) * s.splits;
+  *part = z < cut ? z % s.splits : -1;
+  return z < cut ? z / s.splits : z - cut + cut / s.splits;
+}
+// Part p of the streamed tiles [0, total): *first and the number of them.
+__device__ __forceinline__ int split_range(const AttnShape& s, int total, int p, int* first) {
+  if (p < 0) {
+    *first = 0;
+    return total;
+  }
+  *first = static_cast<int>(static_cast<long long>(total) * p / s.splits);
+  return static_cast<int>(static_cast<long long>(total) * (p + 1) / s.splits) - *first;
+}
+// The partial sums of part p of key tile kt of pair hb = (batch, key head): two matrices
+// (dK then dV) of kBM rows.
+__device__ __forceinline__ float* sink_part_row(const AttnShape& s, int hd, int kt, int hb, int p, int matrix, int row) {
+  const size_t slot = (static_cast<size_t>(kt) * s.Hk * s.B + hb) * s.splits + p;
+  return s.sink_part + ((slot * 2 + matrix) * kBM + row) * hd;
 }
 
 __device__ __forceinline__ size_t row_offset(const Strides3& s, int b, int t, int h) {
@@ -409,6 +471,29 @@ __device__ __forceinline__ void tmem_row_to_global(uint32_t tmem, int warp, int 
     }
     if (write) store_bf16x16(dst + c, v);
   }
+}
+
+// The accumulator columns [col, col + HD) of this thread's lane, times `mult`, as an fp32 row.
+template <int HD>
+__device__ __forceinline__ void tmem_row_to_f32(uint32_t tmem, int warp, int col, float* dst, bool write, float mult) {
+#pragma unroll
+  for (int c = 0; c < HD; c += 16) {
+    uint32_t r[16];
+    tmem_row16(tmem, warp, col + c, r);
+    tmem_wait_ld();
+    reg_fence16(r);
+    if (write)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4*>(dst + c + i) =
+            make_float4(__uint_as_float(r[i]) * mult, __uint_as_float(r[i + 1]) * mult,
+                        __uint_as_float(r[i + 2]) * mult, __uint_as_float(r[i + 3]) * mult);
+  }
+}
+template <int HD>
+__device__ __forceinline__ void zero_row_f32(float* dst) {
+#pragma unroll
+  for (int c = 0; c < HD; c += 4) *reinterpret_cast<float4*>(dst + c) = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 template <int HD>

@@ -441,7 +441,9 @@ __device__ __forceinline__ void dkv_ops(const uint32_t (&vs)[CW], const uint32_t
   }
 }
 
-template <int HD, bool VL, bool GRP>
+// SPLIT: key tiles that hold a sink are cut into parts (split_slot); a part leaves fp32
+// partial sums, which launch_sink_join adds up.
+template <int HD, bool VL, bool GRP, bool SPLIT>
 __global__ void __launch_bounds__(kBBThreads, DkvPass<HD>::CTAS)
     bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                     const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
@@ -468,12 +470,18 @@ __global__ void __launch_bounds__(kBBThreads, DkvPass<HD>::CTAS)
     grouped_order(blockIdx.x, (a.sh.Tk + kBM - 1) / kBM, a.sh.Hk * a.sh.B, a.grp_k, &kt, &hb);
     hk = hb % a.sh.Hk, b = hb / a.sh.Hk;
   }
+  int part = -1;
+  if constexpr (SPLIT) kt = split_slot(a.sh, blockIdx.z, &part);
   SeqRange sr;
   const AttnShape sh = seq_shape<VL>(a.sh, b, &sr);
   const int k0 = kt * kBM;
   int qt_begin;
   const int n = query_tiles(sh, k0, kBM, BN, &qt_begin);  // query tiles that see any of these keys
-  const int total = n * sh.G;  // streamed tiles: n per query head of the group
+  int total = n * sh.G, base = 0;  // streamed tiles: n per query head of the group; SPLIT: from number `base` on
+  if constexpr (SPLIT) total = split_range(sh, total, part, &base);
+  // First query and query head of streamed tile `it`.
+  auto tile_q = [&](int it) { return (qt_begin + (SPLIT ? base + it : it) % n) * BN; };
+  auto tile_h = [&](int it) { return hk * sh.G + (SPLIT ? base + it : it) / n; };
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -511,7 +519,9 @@ __global__ void __launch_bounds__(kBBThreads, DkvPass<HD>::CTAS)
       const size_t off = k_row(sh, sr, key < sh.Tk ? key : 0, hk);
       const __nv_bfloat16* add = wg == 0 ? a.dk_acc : a.dv_acc;
       __nv_bfloat16* dst = (wg == 0 ? a.dk : a.dv) + off;
-      if (key < sh.Tk) {
+      if (SPLIT && part >= 0) {
+        zero_row_f32<HD>(sink_part_row(a.sh, HD, kt, b * sh.Hk + hk, part, wg, key - k0));
+      } else if (key < sh.Tk) {
         if (add) {  // the outputs are the addends
           for (int c = 0; c < HD; c += 8)
             reinterpret_cast<uint4*>(dst + c)[0] = reinterpret_cast<const uint4*>(add + off + c)[0];
@@ -533,8 +543,8 @@ __global__ void __launch_bounds__(kBBThreads, DkvPass<HD>::CTAS)
     constexpr int RPL = BN / 32;
     // L and D of the queries of streamed tile `it`, into registers.
     auto load_stats = [&](int it, float (&raw)[RPL][2]) {
-      const int q0 = (qt_begin + it % n) * BN;
-      const int h = hk * sh.G + it / n;
+      const int q0 = tile_q(it);
+      const int h = tile_h(it);
 #pragma unroll
       for (int k = 0; k < RPL; ++k) {
         const int q = q0 + lane + 32 * k;
@@ -548,8 +558,8 @@ __global__ void __launch_bounds__(kBBThreads, DkvPass<HD>::CTAS)
     int issued = 0;
     for (int it = 0; it < total; ++it) {
       const int s = it % ST;
-      const int q0 = (qt_begin + it % n) * BN;
-      const int h = hk * sh.G + it / n;  // query head of this tile
+      const int q0 = tile_q(it);
+      const int h = tile_h(it);  // query head of this tile
       if (it >= ST && !mbar_wait_warp(&bar_empty[s], ((it / ST) - 1) & 1, &abort_flag)) {
         if (lane == 0) raise_error(a.status, &abort_flag, kDevTimeoutSlotEmpty);
         break;
@@ -689,7 +699,7 @@ __global__ void __launch_bounds__(kBBThreads, DkvPass<HD>::CTAS)
       ok = mbar_wait_warp(&bar_sc_full, it & 1, &abort_flag);
       if (!ok) break;
       tc_fence_after();
-      const int qc = (qt_begin + it % n) * BN + cb;  // first query of this thread's columns
+      const int qc = tile_q(it) + cb;  // first query of this thread's columns
       // Two CTAs per SM (80 registers a thread): the share in two halves of CW/2
       // columns, so half the scores are live at a time.
       constexpr int HW = G::TWO ? CW / 2 : CW, NH = CW / HW;
@@ -729,10 +739,16 @@ __global__ void __launch_bounds__(kBBThreads, DkvPass<HD>::CTAS)
     if (ok) ok = mbar_wait_warp(&bar_acc, 0, &abort_flag);
     if (ok) {
       tc_fence_after();
-      const size_t off = k_row(sh, sr, key_ok ? key : 0, hk);
-      const __nv_bfloat16* add = wg == 0 ? a.dk_acc : a.dv_acc;
-      tmem_row_to_global<HD>(tmem, warp, wg == 0 ? G::C_DK : G::C_DV, (wg == 0 ? a.dk : a.dv) + off, key_ok,
-                             wg == 0 ? sh.scale : 1.f, add ? add + off : nullptr);
+      if (SPLIT && part >= 0) {
+        tmem_row_to_f32<HD>(tmem, warp, wg == 0 ? G::C_DK : G::C_DV,
+                            sink_part_row(a.sh, HD, kt, b * sh.Hk + hk, part, wg, r), key_ok,
+                            wg == 0 ? sh.scale : 1.f);
+      } else {
+        const size_t off = k_row(sh, sr, key_ok ? key : 0, hk);
+        const __nv_bfloat16* add = wg == 0 ? a.dk_acc : a.dv_acc;
+        tmem_row_to_global<HD>(tmem, warp, wg == 0 ? G::C_DK : G::C_DV, (wg == 0 ? a.dk : a.dv) + off, key_ok,
+                               wg == 0 ? sh.scale : 1.f, add ? add + off : nullptr);
+      }
     } else if (threadIdx.x == kBBFirstEwWarp * 32) {
       raise_error(a.status, &abort_flag, kDevTimeoutMma);
     }
@@ -798,10 +814,14 @@ int launch_bwd_hd(const AttnShape& s, const BwdPtrs& p, int* status, cudaStream_
     rc = s.sinks > 0 ? launch_q(&bwd_dq_kernel<HD, VL, false, true>, grid_q)
                      : launch_q(&bwd_dq_kernel<HD, VL, false, false>, grid_q);
   if (rc != kOk) return rc;
-  if constexpr (!VL) {
-    if (args.grp_k < s.Hk * s.B) return launch_k(&bwd_dkdv_kernel<HD, false, true>, dim3(s.Hk * s.B * nk));
+  if (s.splits > 1 && !sink_whole(s)) {
+    rc = launch_k(&bwd_dkdv_kernel<HD, VL, false, true>, dim3(s.Hk, s.B, split_slots(s, nk)));
+    return rc != kOk ? rc : launch_sink_join(s, HD, p.dk, p.dv, p.dk_acc, p.dv_acc, stream);
   }
-  return launch_k(&bwd_dkdv_kernel<HD, VL, false>, grid_k);
+  if constexpr (!VL) {
+    if (args.grp_k < s.Hk * s.B) return launch_k(&bwd_dkdv_kernel<HD, false, true, false>, dim3(s.Hk * s.B * nk));
+  }
+  return launch_k(&bwd_dkdv_kernel<HD, VL, false, false>, grid_k);
 }
 
 }  // namespace

@@ -632,21 +632,24 @@ __device__ __forceinline__ void k_ops(const uint32_t (&vs)[CW], const uint32_t (
 // `l` is the item's sequence (its lengths and mask), `r` where that sequence's rows start.
 struct KItem {
   int hk, b, k0, qt_begin, n, total;  // n query tiles per query head; total = n * G streamed tiles
+  int base, part;                     // SPLIT: a part of a sink tile streams `total` tiles from `base` on (-1: whole)
   AttnShape l;
   SeqRange r;
 };
 
 // Work item w in heaviest-first order (key tile 0 first: the most causal query
 // tiles), key heads fastest; GRP: in locality groups of g (key head, batch) pairs.
-template <bool VL, bool GRP>
+// SPLIT: the parts of the sinks' tiles first (split_slot).
+template <bool VL, bool GRP, bool SPLIT>
 __device__ __forceinline__ KItem k_item(const AttnShape& sh, int w, int bn, int g) {
-  int kt, hb;
+  int kt, hb, part = -1;
   if constexpr (GRP) {
     grouped_order(w, (sh.Tk + kBM - 1) / kBM, sh.Hk * sh.B, g, &kt, &hb);
   } else {
     const int per_kt = sh.Hk * sh.B;
     kt = w / per_kt;
     hb = w - kt * per_kt;
+    if constexpr (SPLIT) kt = split_slot(sh, kt, &part);
   }
   KItem it;
   it.hk = hb % sh.Hk;
@@ -655,6 +658,9 @@ __device__ __forceinline__ KItem k_item(const AttnShape& sh, int w, int bn, int 
   it.l = seq_shape<VL>(sh, it.b, &it.r);
   it.n = query_tiles(it.l, it.k0, kBM, bn, &it.qt_begin);  // query tiles that see any of these keys
   it.total = it.n * sh.G;
+  it.base = 0;
+  it.part = part;
+  if constexpr (SPLIT) it.total = split_range(sh, it.total, part, &it.base);
   return it;
 }
 
@@ -665,7 +671,7 @@ __device__ __forceinline__ KItem k_item(const AttnShape& sh, int w, int bn, int 
 // MMAs of the previous item are done (bar_res_empty), so the reload overlaps the
 // previous item's last tile and epilogue, and the operand MMAs of an item start
 // only once the previous item's accumulators were read out (bar_acc_empty).
-template <int HD, bool VL, bool GRP>
+template <int HD, bool VL, bool GRP, bool SPLIT>
 __global__ void __launch_bounds__(kBBThreads, 1)
     bwdbwd_k_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                     const __grid_constant__ CUtensorMap tm_ddk, const __grid_constant__ CUtensorMap tm_ddv,
@@ -688,8 +694,12 @@ __global__ void __launch_bounds__(kBBThreads, 1)
 
   const AttnShape& sh = a.sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_items = sh.Hk * sh.B * ((sh.Tk + kBM - 1) / kBM);
+  const int key_tiles_all = (sh.Tk + kBM - 1) / kBM;
+  const int n_items = sh.Hk * sh.B * (SPLIT ? split_slots(sh, key_tiles_all) : key_tiles_all);
   const int P = gridDim.x, c = blockIdx.x;
+  // First query and query head of streamed tile `it` of item `w`.
+  auto tile_q = [&](const KItem& w, int it) { return (w.qt_begin + (SPLIT ? w.base + it : it) % w.n) * BN; };
+  auto tile_h = [&](const KItem& w, int it) { return w.hk * sh.G + (SPLIT ? w.base + it : it) / w.n; };
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -731,8 +741,8 @@ __global__ void __launch_bounds__(kBBThreads, 1)
     constexpr int RPL = BN / 32;
     // Per-query statistics of streamed tile `it` of item `w`, into registers.
     auto load_stats = [&](const KItem& w, int it, float (&raw)[RPL][4]) {
-      const int q0 = (w.qt_begin + it % w.n) * BN;
-      const int h = w.hk * sh.G + it / w.n;
+      const int q0 = tile_q(w, it);
+      const int h = tile_h(w, it);
 #pragma unroll
       for (int k = 0; k < RPL; ++k) {
         const int q = q0 + lane + 32 * k;
@@ -748,7 +758,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
     for (int j = 0; ok; ++j) {
       const int wi = snake_item(j, c, P);
       if (wi >= n_items) break;
-      const KItem w = k_item<VL, GRP>(sh, wi, BN, a.grp_k);
+      const KItem w = k_item<VL, GRP, SPLIT>(sh, wi, BN, a.grp_k);
       if (w.total == 0) continue;
       // The previous item's score MMAs no longer read the resident tiles.
       if (ai > 0 && !mbar_wait_warp(&bar_res_empty, (ai - 1) & 1, &abort_flag)) {
@@ -767,8 +777,8 @@ __global__ void __launch_bounds__(kBBThreads, 1)
       load_stats(w, 0, raw_next);
       for (int it = 0; it < w.total; ++it, ++gt) {
         const int s = gt % ST;
-        const int q0 = (w.qt_begin + it % w.n) * BN;
-        const int h = w.hk * sh.G + it / w.n;  // query head of this tile
+        const int q0 = tile_q(w, it);
+        const int h = tile_h(w, it);  // query head of this tile
         if (gt >= ST && !mbar_wait_warp(&bar_empty[s], ((gt / ST) - 1) & 1, &abort_flag)) {
           if (lane == 0) raise_error(a.status, &abort_flag, kDevTimeoutSlotEmpty);
           ok = false;
@@ -832,7 +842,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
     for (int j = 0; ok; ++j) {
       const int wi = snake_item(j, c, P);
       if (wi >= n_items) break;
-      const KItem w = k_item<VL, GRP>(sh, wi, BN, a.grp_k);
+      const KItem w = k_item<VL, GRP, SPLIT>(sh, wi, BN, a.grp_k);
       if (w.total == 0) continue;
       if (!mbar_wait_warp(&bar_res, ai & 1, &abort_flag)) {
         if (lane == 0) raise_error(a.status, &abort_flag, kDevTimeoutTmaFull);
@@ -886,7 +896,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
     for (int j = 0; ok; ++j) {
       const int wi = snake_item(j, c, P);
       if (wi >= n_items) break;
-      const KItem w = k_item<VL, GRP>(sh, wi, BN, a.grp_k);
+      const KItem w = k_item<VL, GRP, SPLIT>(sh, wi, BN, a.grp_k);
       if (w.total == 0) continue;
       for (int it = 0; it < w.total; ++it, ++gt) {
         if (!mbar_wait_warp(&bar_ops_full, gt & 1, &abort_flag)) {
@@ -927,7 +937,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
     for (int j = 0; ok; ++j) {
       const int wi = snake_item(j, c, P);
       if (wi >= n_items) break;
-      const KItem w = k_item<VL, GRP>(sh, wi, BN, a.grp_k);
+      const KItem w = k_item<VL, GRP, SPLIT>(sh, wi, BN, a.grp_k);
       const int key = w.k0 + r;
       const bool key_ok = key < w.l.Tk;
       const int qhi = query_hi(w.l, key), qlo = query_lo(w.l, key);  // queries that see this key
@@ -935,7 +945,10 @@ __global__ void __launch_bounds__(kBBThreads, 1)
       __nv_bfloat16* dst = (wg == 0 ? a.dk2 : a.dv2) + k_row(w.l, w.r, skey, w.hk);
       if (w.total == 0) {
         // No query sees these keys (causal with Tk > Tq): the gradients are zero.
-        if (key_ok) zero_row_global<HD>(dst);
+        if (SPLIT && w.part >= 0)
+          zero_row_f32<HD>(sink_part_row(sh, HD, w.k0 / kBM, w.b * sh.Hk + w.hk, w.part, wg, r));
+        else if (key_ok)
+          zero_row_global<HD>(dst);
         continue;
       }
       // head_dim 128: this item's ddV rows into TMEM, each warpgroup half of the head_dim columns, once
@@ -949,7 +962,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
         warp_arrive(&bar_tres);
       }
       for (int it = 0; it < w.total; ++it, ++gt) {
-        const int qc = (w.qt_begin + it % w.n) * BN + cb;  // first query of this thread's columns
+        const int qc = tile_q(w, it) + cb;  // first query of this thread's columns
         ok = mbar_wait_warp(&bar_sc_full, gt & 1, &abort_flag);
         if (!ok) break;
         tc_fence_after();
@@ -986,7 +999,12 @@ __global__ void __launch_bounds__(kBBThreads, 1)
         break;
       }
       tc_fence_after();
-      tmem_row_to_global<HD>(tmem, warp, wg == 0 ? G::C_DK : G::C_DV, dst, key_ok, wg == 0 ? sc : 1.f);
+      if (SPLIT && w.part >= 0)
+        tmem_row_to_f32<HD>(tmem, warp, wg == 0 ? G::C_DK : G::C_DV,
+                            sink_part_row(sh, HD, w.k0 / kBM, w.b * sh.Hk + w.hk, w.part, wg, r), key_ok,
+                            wg == 0 ? sc : 1.f);
+      else
+        tmem_row_to_global<HD>(tmem, warp, wg == 0 ? G::C_DK : G::C_DV, dst, key_ok, wg == 0 ? sc : 1.f);
       warp_arrive(&bar_acc_empty);  // the accumulators may be overwritten by the next item
       ++ai;
     }
@@ -1080,12 +1098,16 @@ int launch_bwdbwd_hd(const AttnShape& s, const BwdBwdPtrs& p, int passes, int* s
   }
   if (passes & kPassKey) {
     // Persistent: one CTA per SM (at most one per work item).
-    const int items = s.Hk * s.B * ((s.Tk + kBM - 1) / kBM);
+    const int nk = (s.Tk + kBM - 1) / kBM, items = s.Hk * s.B * (s.splits > 1 ? split_slots(s, nk) : nk);
     const dim3 gk(static_cast<unsigned>(items < sm_count() ? items : sm_count()));
-    if constexpr (!VL) {
-      if (grp_k) return launch_k(&bwdbwd_k_kernel<HD, false, true>, gk);
+    if (s.splits > 1) {
+      const HostStatus rc = launch_k(&bwdbwd_k_kernel<HD, VL, false, true>, gk);
+      return rc != kOk ? rc : launch_sink_join(s, HD, p.dk2, p.dv2, nullptr, nullptr, stream);
     }
-    return launch_k(&bwdbwd_k_kernel<HD, VL, false>, gk);
+    if constexpr (!VL) {
+      if (grp_k) return launch_k(&bwdbwd_k_kernel<HD, false, true, false>, gk);
+    }
+    return launch_k(&bwdbwd_k_kernel<HD, VL, false, false>, gk);
   }
   return kOk;
 }

@@ -161,6 +161,12 @@ int validate(const fh_attn_dims* d, AttnShape* out, float scale, int causal, boo
     out->diag = causal == 2 ? d->seq_k - d->seq_q : 0;
     if (d->seq_q + out->diag <= d->window) out->sinks = 0;  // the window hides nothing
   }
+  out->sink_part = static_cast<float*>(d->sink_scratch);
+  out->splits = 1;
+  if (out->sinks > 0 && d->sink_scratch) {
+    if (!aligned16(d->sink_scratch)) return fail(kInvalidArgument, "sink_scratch must be 16-byte aligned");
+    out->splits = sink_splits(*out);
+  }
   return kOk;
 }
 
@@ -248,6 +254,12 @@ const char* fh_status_string(int status) {
     case FH_ERR_NO_DEVICE: return "no CUDA device";
     default: return "unknown status";
   }
+}
+
+long long fh_attn_sink_scratch_floats(const fh_attn_dims* dims, int causal) {
+  AttnShape s;
+  if (validate(dims, &s, 1.f, causal) != kOk) return -1;
+  return sink_part_floats(s, dims->head_dim, sink_splits(s));
 }
 
 int fh_attn_fwd(void* stream, const fh_attn_dims* dims, const void* q, const void* k, const void* v, void* o,

@@ -58,6 +58,11 @@ int launch_bwd(const AttnShape& s, int hd, const BwdPtrs& p, int* status, cudaSt
 enum BwdBwdPass : int { kPassQuery = 1, kPassKey = 2, kPassFwdTangent = 4 };
 int launch_bwdbwd(const AttnShape& s, int hd, const BwdBwdPtrs& p, int passes, int* status, cudaStream_t stream);
 
+// Adds up the partial sums that a key pass with s.splits > 1 left in s.sink_part
+// (sink_join.cu): rows of the key tiles that hold a sink of dk and dv, plus the addends.
+int launch_sink_join(const AttnShape& s, int hd, void* dk, void* dv, const void* dk_acc, const void* dv_acc,
+                     cudaStream_t stream);
+
 // fp32 operands on the CUDA cores (f32.cu): same passes, masks, GQA mapping and
 // layouts as the bf16 kernels; `delta` is written by a rowdot kernel (forward
 // output `o` and `dO`) whenever a pass needs D. No device waits, so no status word.

@@ -113,7 +113,16 @@ typedef struct fh_attn_dims {
   /* First keys that stay visible behind a sliding window (0 = none; needs window > 0):
    * query i also sees keys j < sinks with j <= diag_i. Per sequence in a packed batch. */
   int32_t sinks;
+  /* Optional scratch of the bf16 backward and double backward with sinks, 16-byte
+   * aligned, fh_attn_sink_scratch_floats(dims, causal) floats: a key tile that holds a
+   * sink is seen by every query, and with scratch its work is cut into parts that run
+   * side by side. NULL: whole, slower where the window is short, the same result up to
+   * the order of its sums. */
+  void* sink_scratch;
 } fh_attn_dims;
+
+/* Floats of fh_attn_dims.sink_scratch (0: it would not be used; -1: invalid dims). */
+long long fh_attn_sink_scratch_floats(const fh_attn_dims* dims, int causal);
 
 /* Forward: o = softmax(scale * q k^T + mask) v, lse = logsumexp(scale * q k^T + mask).
  * Replaces the cuDNN forward with residuals, flash_hog/jax/_attention_impl.py:224-239
