@@ -58,6 +58,8 @@ EXPORTED_SYMBOLS = (
     "fh_embed_bwd",
     "fh_embed_bwd_bwd",
     "fh_dropout",
+    "fh_policy_stats_floats",
+    "fh_policy_scratch_floats",
     "fh_policy_fwd",
     "fh_policy_bwd",
     "fh_policy_bwd_bwd",
@@ -146,9 +148,11 @@ def lib() -> ctypes.CDLL:
     h.fh_embed_bwd.argtypes = [vp, i32, i32, i32, i32, vp, vp, f32, ll, vp, vp]
     h.fh_embed_bwd_bwd.argtypes = [vp, i32, i32, i32, i32, vp, vp, f32, ll, vp]
     h.fh_dropout.argtypes = [vp, ll, i32, vp, i32, vp, i32, vp, vp, ctypes.c_uint, i32]
+    for f in (h.fh_policy_stats_floats, h.fh_policy_scratch_floats):
+        f.argtypes, f.restype = [i32, i32], ll
     h.fh_policy_fwd.argtypes = [vp, i32, i32, i32, ll] + [vp] * 6 + [f32] * 4 + [vp] * 3
     h.fh_policy_bwd.argtypes = [vp, i32, i32, i32, ll] + [vp] * 5
-    h.fh_policy_bwd_bwd.argtypes = [vp, i32, i32, i32, ll] + [vp] * 7
+    h.fh_policy_bwd_bwd.argtypes = [vp, i32, i32, i32, ll] + [vp] * 8
     h.fh_device_status.argtypes = [vp, ctypes.POINTER(ctypes.c_int)]
     h.fh_status_string.argtypes = [i32]
     h.fh_status_string.restype = ctypes.c_char_p
@@ -588,6 +592,11 @@ def _policy_args(z, actions, *vectors):
     return _GELU_DTYPES[z.dtype], rows, vocab, z.stride(0) if rows > 1 else vocab
 
 
+def policy_stats(z) -> torch.Tensor:
+    """Uninitialised ``stats`` of ``policy_fwd`` for these logits."""
+    return torch.empty(int(lib().fh_policy_stats_floats(z.shape[0], z.shape[1])), dtype=torch.float32, device=z.device)
+
+
 @_on_device
 def policy_fwd(z, actions, old, adv, ref, weights, clip_low: float, clip_high: float, kl_coef: float,
                normalizer: float, lp, loss, stats) -> None:
@@ -617,8 +626,10 @@ def policy_bwd_bwd(z, actions, stats, g, u, gz, gg) -> None:
     for x in (u, gz):
         if x.dtype != z.dtype or not x.is_contiguous() or x.shape != z.shape:
             raise ValueError("u and gz are contiguous tensors of the logits' shape and dtype")
+    n = int(lib().fh_policy_scratch_floats(z.shape[0], z.shape[1]))
+    scratch = torch.empty(n, dtype=torch.float32, device=z.device) if n else None
     _check("fh_policy_bwd_bwd", lib().fh_policy_bwd_bwd(_stream(z.device), *args, _ptr(z), _ptr(actions), _ptr(stats),
-                                                       _ptr(g), _ptr(u), _ptr(gz), _ptr(gg)))
+                                                       _ptr(g), _ptr(u), _ptr(gz), _ptr(gg), _ptr(scratch)))
 
 
 def launch_count() -> int:

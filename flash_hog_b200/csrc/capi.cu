@@ -627,8 +627,8 @@ int fh_dropout(void* stream, long long n, int x_dtype, const void* x, int res_dt
   if (injected("fh_dropout")) return FH_ERR_INJECTED;
   g_last_error[0] = 0;
   auto dtype_ok = [](int d) { return d == 0 || d == 1; };
-  if (n < 0 || !dtype_ok(x_dtype) || !dtype_ok(y_dtype) || (res && !dtype_ok(res_dtype)) || limit < 0 || limit > 65536)
-    return fail(FH_ERR_INVALID_ARGUMENT, "dropout: n >= 0, dtypes 0 (fp32) or 1 (bf16), limit in [0, 65536]");
+  if (n < 0 || n > (1ll << 42) || !dtype_ok(x_dtype) || !dtype_ok(y_dtype) || (res && !dtype_ok(res_dtype)) || limit < 0 || limit > 65536)
+    return fail(FH_ERR_INVALID_ARGUMENT, "dropout: n in [0, 2^42], dtypes 0 (fp32) or 1 (bf16), limit in [0, 65536]");
   if (res && y_dtype != (x_dtype & res_dtype))
     return fail(FH_ERR_INVALID_ARGUMENT, "dropout: with a residual y is bf16 where both inputs are, else fp32");
   if (n == 0) return FH_OK;
@@ -646,9 +646,21 @@ static int policy_check(int dtype, int rows, int vocab, long long ld, const void
   g_last_error[0] = 0;
   if (rows < 0 || vocab < 1 || ld < vocab || (dtype != 0 && dtype != 1))
     return fail(FH_ERR_INVALID_ARGUMENT, "policy: rows >= 0, vocab >= 1, ld >= vocab, dtype 0 (fp32) or 1 (bf16)");
-  if (!stats || (rows > 0 && (!z || !actions)))
-    return fail(FH_ERR_INVALID_ARGUMENT, "policy: logits, actions and stats are required");
+  if (!all_aligned(stats) || (rows > 0 && (!z || !actions)))
+    return fail(FH_ERR_INVALID_ARGUMENT, "policy: logits, actions and (16-byte aligned) stats are required");
   return kOk;
+}
+
+long long fh_policy_stats_floats(int rows, int vocab) {
+  g_last_error[0] = 0;
+  if (rows < 0 || vocab < 1) return -1;
+  return policy_stats_floats(rows, vocab);
+}
+
+long long fh_policy_scratch_floats(int rows, int vocab) {
+  g_last_error[0] = 0;
+  if (rows < 0 || vocab < 1) return -1;
+  return policy_scratch_floats(rows, vocab);
 }
 
 int fh_policy_fwd(void* stream, int dtype, int rows, int vocab, long long ld, const void* z, const long long* actions,
@@ -666,16 +678,18 @@ int fh_policy_fwd(void* stream, int dtype, int rows, int vocab, long long ld, co
   return launch_policy(0,
                        PolicyArgs{dtype == 1, rows, vocab, ld, z, actions, old, adv, ref, weights, clip_low, clip_high,
                                   kl_coef, normalizer, lp, loss, stats},
-                       nullptr, nullptr, nullptr, nullptr, st);
+                       nullptr, nullptr, nullptr, nullptr, nullptr, st);
 }
 
 static int policy_grad(int op, void* stream, int dtype, int rows, int vocab, long long ld, const void* z,
                        const long long* actions, const float* stats, const float* g, const void* u, void* out,
-                       float* gg) {
+                       float* gg, float* scratch) {
   int rc = policy_check(dtype, rows, vocab, ld, z, actions, stats);
   if (rc != kOk || rows == 0) return rc;
   if (!g || !out || (op == 2 && (!u || !gg)))
     return fail(FH_ERR_INVALID_ARGUMENT, "policy: g and the outputs (and u) are required");
+  if (op == 2 && !scratch && policy_scratch_floats(rows, vocab) > 0)
+    return fail(FH_ERR_INVALID_ARGUMENT, "policy: these sizes need scratch (fh_policy_scratch_floats)");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if ((rc = select_stream_device(st)) != kOk) return rc;
   PolicyArgs a{};
@@ -686,20 +700,20 @@ static int policy_grad(int op, void* stream, int dtype, int rows, int vocab, lon
   a.z = z;
   a.actions = actions;
   a.stats = const_cast<float*>(stats);
-  return launch_policy(op, a, g, u, out, gg, st);
+  return launch_policy(op, a, g, u, out, gg, scratch, st);
 }
 
 int fh_policy_bwd(void* stream, int dtype, int rows, int vocab, long long ld, const void* z, const long long* actions,
                   const float* stats, const float* g, void* dz) {
   if (injected("fh_policy_bwd")) return FH_ERR_INJECTED;
-  return policy_grad(1, stream, dtype, rows, vocab, ld, z, actions, stats, g, nullptr, dz, nullptr);
+  return policy_grad(1, stream, dtype, rows, vocab, ld, z, actions, stats, g, nullptr, dz, nullptr, nullptr);
 }
 
 int fh_policy_bwd_bwd(void* stream, int dtype, int rows, int vocab, long long ld, const void* z,
                       const long long* actions, const float* stats, const float* g, const void* u, void* gz,
-                      float* gg) {
+                      float* gg, float* scratch) {
   if (injected("fh_policy_bwd_bwd")) return FH_ERR_INJECTED;
-  return policy_grad(2, stream, dtype, rows, vocab, ld, z, actions, stats, g, u, gz, gg);
+  return policy_grad(2, stream, dtype, rows, vocab, ld, z, actions, stats, g, u, gz, gg, scratch);
 }
 
 int fh_device_status(void* stream, int* code) {

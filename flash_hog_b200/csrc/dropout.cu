@@ -45,9 +45,36 @@ __device__ __forceinline__ uint4 philox(unsigned long long block, unsigned sub, 
   return make_uint4(c0, c1, c2, c3);
 }
 
-// TR = void: no residual. Each thread takes whole Philox blocks of eight elements; the
-// last n % 8 elements, and all of them when a pointer is not 16-byte aligned (VEC false),
-// go one by one.
+// keep(k) of a Philox block's eight draws: draw k is the low (even k) or high half of word
+// k / 2. Compared in the upper half of a word, where the other draw's bits do not count.
+struct Keep {
+  uint32_t words[4];
+  uint32_t limit16;  // limit << 16; all dropped (limit 65536) is the caller's case
+  __device__ __forceinline__ bool operator()(int k) const {
+    return (k & 1 ? words[k >> 1] : words[k >> 1] << 16) >= limit16;
+  }
+};
+
+// N elements' values as loaded, converted when used.
+template <typename T>
+struct Eight {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int q = 0; q < static_cast<int>(sizeof(T) / 2); ++q) v[q] = reinterpret_cast<const uint4*>(p)[q];
+  }
+  __device__ __forceinline__ void get(float (&x)[kDraws]) const {
+    load_vec<T, kDraws>(reinterpret_cast<const T*>(v), x);
+  }
+};
+template <>
+struct Eight<void> {};
+
+// TR = void: no residual. Each thread takes kDropBlocks whole Philox blocks of eight
+// elements, whose loads are issued before the draws are computed. The last blocks, and all
+// when a pointer is not 16-byte aligned (VEC false), go element by element.
+constexpr int kDropBlocks = 2;
+
 template <typename TI, typename TR, typename TO, bool VEC>
 __global__ void __launch_bounds__(kDropThreads) dropout_kernel(long long n, const TI* __restrict__ x,
                                                                const TR* __restrict__ res, TO* __restrict__ y,
@@ -55,35 +82,50 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(long long n, cons
                                                                unsigned limit, float factor) {
   constexpr bool RES = !std::is_same<TR, void>::value;
   const unsigned long long key = static_cast<unsigned long long>(*seed);
-  const long long blocks = (n + kDraws - 1) / kDraws;
-  for (long long b = static_cast<long long>(blockIdx.x) * kDropThreads + threadIdx.x; b < blocks;
-       b += static_cast<long long>(gridDim.x) * kDropThreads) {
-    const long long i0 = b * kDraws;
+  const long long b0 = static_cast<long long>(blockIdx.x) * (kDropThreads * kDropBlocks) + threadIdx.x;
+  auto draw = [&](long long b) {
     const uint4 w = philox(static_cast<unsigned long long>(b), sub, key);
-    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-    auto keep = [&](int k) { return ((words[k >> 1] >> (16 * (k & 1))) & 0xffffu) >= limit; };
-    if (VEC && i0 + kDraws <= n) {
+    return Keep{{w.x, w.y, w.z, w.w}, limit << 16};
+  };
+  if (VEC && limit < 65536u && (b0 + (kDropBlocks - 1) * kDropThreads + 1) * kDraws <= n) {
+    Eight<TI> xv[kDropBlocks];
+    [[maybe_unused]] Eight<TR> rv[kDropBlocks];
+#pragma unroll
+    for (int q = 0; q < kDropBlocks; ++q) {
+      const long long i0 = (b0 + q * kDropThreads) * kDraws;
+      xv[q].load(x + i0);
+      if constexpr (RES) rv[q].load(res + i0);
+    }
+#pragma unroll
+    for (int q = 0; q < kDropBlocks; ++q) {
+      const long long b = b0 + q * kDropThreads;
+      const Keep keep = draw(b);
       float v[kDraws], o[kDraws];
-      load_vec<TI, kDraws>(x + i0, v);
+      xv[q].get(v);
       if constexpr (RES) {
         float r[kDraws];
-        load_vec<TR, kDraws>(res + i0, r);
+        rv[q].get(r);
 #pragma unroll
         for (int k = 0; k < kDraws; ++k) o[k] = keep(k) ? fmaf(v[k], factor, r[k]) : r[k];
       } else {
 #pragma unroll
         for (int k = 0; k < kDraws; ++k) o[k] = keep(k) ? v[k] * factor : 0.f;
       }
-      store_vec<TO, kDraws>(y + i0, o);
-    } else {
+      store_vec<TO, kDraws>(y + b * kDraws, o);
+    }
+    return;
+  }
+  for (int q = 0; q < kDropBlocks; ++q) {
+    const long long b = b0 + q * kDropThreads, i0 = b * kDraws;
+    if (i0 >= n) return;
+    const Keep keep = draw(b);
 #pragma unroll
-      for (int k = 0; k < kDraws; ++k) {
-        if (i0 + k >= n) continue;
-        float o = 0.f;
-        if constexpr (RES) o = to_f32(res[i0 + k]);
-        if (keep(k)) o = fmaf(to_f32(x[i0 + k]), factor, o);
-        y[i0 + k] = from_f32<TO>(o);
-      }
+    for (int k = 0; k < kDraws; ++k) {
+      if (i0 + k >= n) continue;
+      float o = 0.f;
+      if constexpr (RES) o = to_f32(res[i0 + k]);
+      if (limit < 65536u && keep(k)) o = fmaf(to_f32(x[i0 + k]), factor, o);
+      y[i0 + k] = from_f32<TO>(o);
     }
   }
 }
@@ -92,8 +134,8 @@ template <typename TI, typename TR, typename TO>
 int launch_typed(long long n, const void* x, const void* res, void* y, const long long* seed, unsigned sub,
                  unsigned limit, float factor, cudaStream_t stream) {
   const bool vec = vec_aligned(x) && vec_aligned(res) && vec_aligned(y);
-  const long long blocks = ((n + kDraws - 1) / kDraws + kDropThreads - 1) / kDropThreads, cap = 1ll << 30;
-  const unsigned grid = static_cast<unsigned>(blocks < cap ? blocks : cap);
+  constexpr long long kPerBlock = static_cast<long long>(kDropThreads) * kDropBlocks * kDraws;
+  const unsigned grid = static_cast<unsigned>((n + kPerBlock - 1) / kPerBlock);
   if (vec)
     dropout_kernel<TI, TR, TO, true><<<grid, kDropThreads, 0, stream>>>(
         n, static_cast<const TI*>(x), static_cast<const TR*>(res), static_cast<TO*>(y), seed, sub, limit, factor);

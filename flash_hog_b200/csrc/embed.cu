@@ -40,36 +40,54 @@ namespace {
 
 constexpr int kLookupThreads = 256;
 
-// `lanes` (a power of two up to kLookupThreads) threads per token. A token outside
-// [0, vocab) gives `oob` in every element; token `skip` gives zeros (-1: none).
+// `lanes` (a power of two up to kLookupThreads) threads per token, each block kLookupRows
+// times as many tokens as it has such groups: their ids are loaded together, then their
+// rows, so that a group has several rows in flight. A token outside [0, vocab) gives `oob`
+// in every element; token `skip` gives zeros (-1: none).
+constexpr int kLookupRows = 4;
+
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kLookupThreads) embed_lookup_kernel(long long n, long long vocab, int dim, int lanes_log2,
-                                                                      const long long* __restrict__ tokens,
-                                                                      const T* __restrict__ w, float scale,
-                                                                      long long skip, float oob, T* __restrict__ y) {
+__global__ void __launch_bounds__(kLookupThreads)
+    embed_lookup_kernel(long long n, long long vocab, int dim, int lanes_log2, const long long* __restrict__ tokens,
+                        const T* __restrict__ w, float scale, long long skip, float oob, T* __restrict__ y) {
   constexpr int E = VEC ? 16 / sizeof(T) : 1;
-  const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
-  const int per_block = kLookupThreads >> lanes_log2, nv = dim / E;
-  for (long long i = static_cast<long long>(blockIdx.x) * per_block + (threadIdx.x >> lanes_log2); i < n;
-       i += static_cast<long long>(gridDim.x) * per_block) {
-    const long long t = tokens[i];
-    T* out = y + i * dim;
-    const bool outside = t < 0 || t >= vocab;
-    if (outside || t == skip) {
-      float v[E];
+  const int lane = threadIdx.x & ((1 << lanes_log2) - 1);
+  const int groups = kLookupThreads >> lanes_log2, nv = dim / E;
+  const long long i0 = static_cast<long long>(blockIdx.x) * groups * kLookupRows + (threadIdx.x >> lanes_log2);
+  long long t[kLookupRows];
+  bool plain = i0 + (kLookupRows - 1) * groups < n;  // whole group of rows, every token in the table
 #pragma unroll
-      for (int k = 0; k < E; ++k) v[k] = outside ? oob : 0.f;
-      for (int c = lane; c < nv; c += lanes) store_vec<T, E>(out + c * E, v);
-      continue;
+  for (int r = 0; r < kLookupRows; ++r) {
+    const long long i = i0 + r * groups;
+    t[r] = i < n ? tokens[i] : -1;
+    plain = plain && t[r] >= 0 && t[r] < vocab && t[r] != skip;
+  }
+  if (plain) {
+    for (int c = lane; c < nv; c += 1 << lanes_log2) {
+      float v[kLookupRows][E];
+#pragma unroll
+      for (int r = 0; r < kLookupRows; ++r) load_vec<T, E>(w + t[r] * dim + c * E, v[r]);
+#pragma unroll
+      for (int r = 0; r < kLookupRows; ++r) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[r][k] *= scale;
+        store_vec<T, E>(y + (i0 + r * groups) * dim + c * E, v[r]);
+      }
     }
-    const T* row = w + t * dim;
-#pragma unroll 4
-    for (int c = lane; c < nv; c += lanes) {
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < kLookupRows; ++r) {
+    const long long i = i0 + r * groups;
+    if (i >= n) return;
+    const bool outside = t[r] < 0 || t[r] >= vocab, none = outside || t[r] == skip;
+    const T* row = w + (none ? 0 : t[r]) * dim;
+    for (int c = lane; c < nv; c += 1 << lanes_log2) {
       float v[E];
       load_vec<T, E>(row + c * E, v);
 #pragma unroll
-      for (int k = 0; k < E; ++k) v[k] *= scale;
-      store_vec<T, E>(out + c * E, v);
+      for (int k = 0; k < E; ++k) v[k] = none ? (outside ? oob : 0.f) : v[k] * scale;
+      store_vec<T, E>(y + i * dim + c * E, v);
     }
   }
 }
@@ -230,6 +248,24 @@ struct SumArgs {
   float* tail;  // [chunks][dim]: sum of the run that began in the chunk and goes on after it
 };
 
+// 16 bytes, or one element, as loaded: converted only when it is used, so that all loads
+// of a batch of rows are issued before the first wait.
+template <typename T, bool VEC>
+struct Raw {
+  static constexpr int E = VEC ? 16 / sizeof(T) : 1;
+  alignas(VEC ? 16 : sizeof(T)) T v[E];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
+    else v[0] = *p;
+  }
+  __device__ __forceinline__ void add_to(float (&acc)[E]) const {
+    float x[E];
+    load_vec<T, E>(v, x);
+#pragma unroll
+    for (int k = 0; k < E; ++k) acc[k] += x[k];
+  }
+};
+
 // One chunk (blockIdx.x) x one tile of kSumThreads * E columns (blockIdx.y).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(const SumArgs a, const T* __restrict__ dy,
@@ -237,25 +273,25 @@ __global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(const SumArgs a,
   constexpr int E = VEC ? 16 / sizeof(T) : 1;
   const int col = (blockIdx.y * kSumThreads + threadIdx.x) * E;
   const int j0 = blockIdx.x * a.chunk, j1 = min(j0 + a.chunk, a.n);
-  if (col >= a.dim) return;
   const unsigned vocab = static_cast<unsigned>(a.vocab);
+  if (col >= a.dim || a.key[j0] == vocab) return;
   bool from_before = j0 > 0 && a.key[j0 - 1] == a.key[j0];
   float acc[E];
 #pragma unroll
   for (int k = 0; k < E; ++k) acc[k] = 0.f;
   for (int j = j0; j < j1; j += kAhead) {
     unsigned key[kAhead + 1];
-    float v[kAhead][E];
+    Raw<T, VEC> v[kAhead];
 #pragma unroll
     for (int u = 0; u <= kAhead; ++u) key[u] = j + u < a.n ? a.key[j + u] : vocab;
+    // Entries past the chunk or without a gradient load some row of dy all the same: a
+    // load under a condition would wait for the one before it.
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (j + u < j1 && key[u] != vocab) load_vec<T, E>(dy + static_cast<long long>(a.pos[j + u]) * a.dim + col, v[u]);
+    for (int u = 0; u < kAhead; ++u) v[u].load(dy + static_cast<long long>(a.pos[min(j + u, a.n - 1)]) * a.dim + col);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (j + u >= j1 || key[u] == vocab) continue;
-#pragma unroll
-      for (int k = 0; k < E; ++k) acc[k] += v[u][k];
+      v[u].add_to(acc);
       const bool ends = key[u + 1] != key[u];  // the list's end counts as another key
       if (!ends && j + u + 1 < j1) continue;
       if (from_before) {
@@ -274,44 +310,104 @@ __global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(const SumArgs a,
   }
 }
 
-// The run that begins in chunk blockIdx.x and goes on after it, if there is one.
+// Partial sums [p0, p1) of the run that begins in chunk c0, in order: number 0 is c0's
+// tail, number q > 0 the head of chunk c0 + q.
+template <int E>
+__device__ __forceinline__ void add_parts(const SumArgs& a, int c0, int p0, int p1, int col, float (&acc)[E]) {
+  for (int p = p0; p < p1; p += 4) {
+    alignas(16) float x[4][E];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int q = min(p + u, p1 - 1);
+      const float* src = (q == 0 ? a.tail : a.head) + static_cast<long long>(c0 + q) * a.dim + col;
+      load_vec<float, E>(src, x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (p + u < p1)
+#pragma unroll
+        for (int k = 0; k < E; ++k) acc[k] += x[u][k];
+  }
+}
+
+// The runs that begin in one of the kJoinWarps chunks of blockIdx.x and go on after it, one
+// tile of 32 * E columns (blockIdx.y). Each warp looks at its chunk's run and adds it up if
+// it spans a few chunks; the block adds up the longer ones together, each warp a stretch of
+// the run, the warps' sums in order.
+constexpr int kJoinWarps = 8;
+constexpr int kJoinAlone = 8;
+
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kSumThreads) embed_join_kernel(const SumArgs a, T* __restrict__ dw) {
+__global__ void __launch_bounds__(32 * kJoinWarps) embed_join_kernel(const SumArgs a, T* __restrict__ dw) {
   constexpr int E = VEC ? 16 / sizeof(T) : 1;
-  const int col = (blockIdx.y * kSumThreads + threadIdx.x) * E;
-  const int j0 = blockIdx.x * a.chunk, next = j0 + a.chunk;
-  if (col >= a.dim || next >= a.n) return;
-  const unsigned key = a.key[next - 1];
-  if (key == static_cast<unsigned>(a.vocab) || a.key[next] != key) return;
-  if (j0 > 0 && a.key[j0 - 1] == key) return;  // it began before this chunk
-  // Its last chunk: the one with the last entry of the run (binary search in the sorted list).
-  int lo = next, hi = a.n - 1;
-  while (lo < hi) {
-    const int mid = lo + (hi - lo + 1) / 2;
-    if (a.key[mid] == key) lo = mid;
-    else hi = mid - 1;
-  }
-  const int c1 = lo / a.chunk;
-  float acc[E];
-  load_vec<float, E>(a.tail + static_cast<long long>(blockIdx.x) * a.dim + col, acc);
-#pragma unroll 8
-  for (int c = blockIdx.x + 1; c <= c1; ++c) {
-    float v[E];
-    load_vec<float, E>(a.head + static_cast<long long>(c) * a.dim + col, v);
+  __shared__ float parts[kJoinWarps][32 * E];
+  __shared__ int spans[kJoinWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = (blockIdx.y * 32 + lane) * E;
+  const bool ok = col < a.dim;
+  auto finish = [&](unsigned key, float (&acc)[E]) {
 #pragma unroll
-    for (int k = 0; k < E; ++k) acc[k] += v[k];
+    for (int k = 0; k < E; ++k) acc[k] *= a.scale;
+    store_vec<T, E>(dw + static_cast<long long>(key) * a.dim + col, acc);
+  };
+  // Chunks that the run of this warp's chunk spans; 0 where none begins here and goes on.
+  const int c = blockIdx.x * kJoinWarps + warp;
+  int span = 0;
+  if (c + 1 < a.chunks) {
+    const int j0 = c * a.chunk, next = j0 + a.chunk;
+    const unsigned key = a.key[next - 1];
+    if (key != static_cast<unsigned>(a.vocab) && a.key[next] == key && (j0 == 0 || a.key[j0 - 1] != key)) {
+      // Whether the run fills chunk c + 1 + l and reaches the next, 32 chunks at a time.
+      for (span = 1;; span += 32) {
+        const long long after = static_cast<long long>(c + span + lane + 1) * a.chunk;
+        const unsigned on = __ballot_sync(0xffffffffu, after < a.n && a.key[after] == key);
+        if (on != 0xffffffffu) {
+          span += __ffs(~on);
+          break;
+        }
+      }
+    }
   }
+  if (lane == 0) spans[warp] = span;
+  if (span > 0 && span <= kJoinAlone && ok) {
+    float acc[E];
 #pragma unroll
-  for (int k = 0; k < E; ++k) acc[k] *= a.scale;
-  store_vec<T, E>(dw + static_cast<long long>(key) * a.dim + col, acc);
+    for (int k = 0; k < E; ++k) acc[k] = 0.f;
+    add_parts<E>(a, c, 0, span, col, acc);
+    finish(a.key[c * a.chunk + a.chunk - 1], acc);
+  }
+  __syncthreads();
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const int n = spans[w], c0 = blockIdx.x * kJoinWarps + w;
+    if (n <= kJoinAlone) continue;
+    const int per = (n + kJoinWarps - 1) / kJoinWarps, p0 = min(warp * per, n), p1 = min(p0 + per, n);
+    float acc[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) acc[k] = 0.f;
+    if (ok) add_parts<E>(a, c0, p0, p1, col, acc);
+#pragma unroll
+    for (int k = 0; k < E; ++k) parts[warp][k * 32 + lane] = acc[k];
+    __syncthreads();
+    if (warp == 0 && ok) {
+#pragma unroll
+      for (int g = 1; g < kJoinWarps; ++g)
+#pragma unroll
+        for (int k = 0; k < E; ++k) acc[k] += parts[g][k * 32 + lane];
+      finish(a.key[c0 * a.chunk + a.chunk - 1], acc);
+    }
+    __syncthreads();
+  }
 }
 
 // Sorted entries per chunk: small enough that the chunks of a short list still fill the
-// GPU, at most 32, where the partial sums of a list with long runs (at most two fp32 rows
-// a chunk) are a small part of the chunk's own rows.
+// GPU, and from 32 on larger only for long lists: long runs leave at most two fp32 rows of
+// partial sums a chunk, a small part of the chunk's own 32 rows, and the join of a run
+// reads them all (500000 tokens with a run of 52800, dim 64: sums and join 85 us in chunks
+// of 32, 66 us of 128).
 int embed_chunk(int n) {
   int c = 8;
   while (c < 32 && n / c > 4 * 148) c *= 2;
+  while (c >= 32 && c < 128 && n / c > 32 * 148) c *= 2;
   return c;
 }
 
@@ -332,8 +428,8 @@ int launch_embed_lookup(bool bf16, long long n, int vocab, int dim, const long l
   // Threads per token: enough for one 16-byte access each, or the whole block.
   int lg = 0;
   while ((1 << lg) < per_row && (1 << lg) < kLookupThreads) ++lg;
-  const long long blocks = (n + (kLookupThreads >> lg) - 1) / (kLookupThreads >> lg), cap = 64ll * sm_count();
-  const unsigned grid = static_cast<unsigned>(blocks < cap ? blocks : cap);
+  const int rows = (kLookupThreads >> lg) * kLookupRows;
+  const unsigned grid = static_cast<unsigned>((n + rows - 1) / rows);
 #define FH_LOOKUP(T, V)                                                                                           \
   embed_lookup_kernel<T, V><<<grid, kLookupThreads, 0, stream>>>(n, vocab, dim, lg, tokens, static_cast<const T*>(w), \
                                                                  scale, skip, oob, static_cast<T*>(y))
@@ -372,10 +468,10 @@ int launch_embed_grad(bool bf16, int n, int vocab, int dim, const long long* tok
   if (ensure_smem_limit(reinterpret_cast<const void*>(&embed_sort_kernel),
                         (kSortWarps + 1) * (1 << kMaxDigitBits) * 4) != kOk)
     return kLaunchFailed;
-  // Clusters that fill: one more CTA than SMs are left, in whole clusters, or fewer when
-  // there is little to fill.
+  // CTAs that fill: two per SM, or fewer when there is little to fill. (With one per SM
+  // the clusters of a GPC share its SMs unevenly: 98 MB took 26 us.)
   const long long want = (so.fill_vecs + 8ll * kSortThreads - 1) / (8ll * kSortThreads) + 1;
-  const long long most = sm_count();
+  const long long most = 2 * sm_count() - kSortCluster;
   const long long ctas = want < most ? want : most;
   const unsigned grid = static_cast<unsigned>(kSortCluster * (1 + (ctas + kSortCluster - 1) / kSortCluster));
   embed_sort_kernel<<<grid, kSortThreads, smem, stream>>>(so);
@@ -396,12 +492,14 @@ int launch_embed_grad(bool bf16, int n, int vocab, int dim, const long long* tok
   const bool vec = dim % e == 0 && vec_aligned(dy) && vec_aligned(dw);
   const int cols = kSumThreads * (vec ? e : 1);
   const dim3 g(su.chunks, (dim + cols - 1) / cols);
+  const int join_cols = 32 * (vec ? e : 1);
+  const dim3 gj((su.chunks + kJoinWarps - 1) / kJoinWarps, (dim + join_cols - 1) / join_cols);
 #define FH_SUM(T, V)                                                                                              \
   do {                                                                                                            \
     embed_sum_kernel<T, V><<<g, kSumThreads, 0, stream>>>(su, static_cast<const T*>(dy), static_cast<T*>(dw));    \
     if (after_launch() != kOk) return kLaunchFailed;                                                              \
     if (su.chunks > 1) {                                                                                          \
-      embed_join_kernel<T, V><<<g, kSumThreads, 0, stream>>>(su, static_cast<T*>(dw));                            \
+      embed_join_kernel<T, V><<<gj, 32 * kJoinWarps, 0, stream>>>(su, static_cast<T*>(dw));                            \
       return after_launch();                                                                                      \
     }                                                                                                             \
     return kOk;                                                                                                   \

@@ -135,10 +135,13 @@ struct PolicyArgs {
   const long long* actions;
   const float *old, *adv, *ref, *weights;  // ref: with beta; weights null: all 1
   float clip_low, clip_high, beta, normalizer;  // normalizer 0: the sum of the weights
-  float *lp, *loss, *stats;  // stats: 6 rows + 1 floats
+  float *lp, *loss, *stats;  // stats: policy_stats_floats, 16-byte aligned
 };
-int launch_policy(int op, const PolicyArgs& a, const float* g, const void* u, void* out, float* gg,
+// scratch: policy_scratch_floats, op 2.
+int launch_policy(int op, const PolicyArgs& a, const float* g, const void* u, void* out, float* gg, float* scratch,
                   cudaStream_t stream);
+long long policy_stats_floats(int rows, int vocab);
+long long policy_scratch_floats(int rows, int vocab);
 
 // Checks the kernel launch just made (cudaGetLastError) and, if it was queued,
 // counts it for fh_launch_count(). Returns kOk or kLaunchFailed.

@@ -371,7 +371,7 @@ class _PolicyLoss(torch.autograd.Function):
         rows = z.shape[0]
         lp = torch.empty(rows, dtype=torch.float32, device=z.device)
         loss = torch.empty((), dtype=torch.float32, device=z.device)
-        stats = torch.empty(6 * rows + 1, dtype=torch.float32, device=z.device)
+        stats = _capi.policy_stats(z)
         _capi.policy_fwd(z, actions, old, adv, ref, weights, clip_low, clip_high, kl_coef, normalizer, lp, loss, stats)
         ctx.save_for_backward(z, actions, stats)
         ctx.mark_non_differentiable(lp)

@@ -364,10 +364,14 @@ int fh_dropout(void* stream, long long n, int x_dtype, const void* x, int res_dt
  *   loss = sum w l / N, N = normalizer if that is > 0, else sum w (loss 0 where N = 0).
  * A row of weight 0 is not read: it gives lp = 0 and zero gradients whatever it holds. An
  * action outside [0, vocab) in another row gives NaN. rows may be 0.
- *  - fh_policy_fwd: lp[r], loss[0] and `stats` (6 rows + 1 floats, for the passes below).
+ *  - fh_policy_fwd: lp[r], loss[0] and `stats` (fh_policy_stats_floats(rows, vocab) floats,
+ *    16-byte aligned, for the passes below, which only read it). Two launches.
  *  - fh_policy_bwd: dz = g dloss/dz (z's dtype, contiguous); g: fp32, device memory.
  *  - fh_policy_bwd_bwd: given the cotangent u of dz (z's dtype, contiguous): gz, the
- *    gradient of <u, dz> by z, and gg[r], whose sum is the one by g. */
+ *    gradient of <u, dz> by z, and gg[r], whose sum is the one by g. `scratch`:
+ *    fh_policy_scratch_floats(rows, vocab) floats (NULL where that is 0). */
+long long fh_policy_stats_floats(int rows, int vocab);
+long long fh_policy_scratch_floats(int rows, int vocab);
 int fh_policy_fwd(void* stream, int dtype, int rows, int vocab, long long ld, const void* z, const long long* actions,
                   const float* old, const float* adv, const float* ref, const float* weights, float clip_low,
                   float clip_high, float kl_coef, float normalizer, float* lp, float* loss, float* stats);
@@ -375,7 +379,7 @@ int fh_policy_bwd(void* stream, int dtype, int rows, int vocab, long long ld, co
                   const float* stats, const float* g, void* dz);
 int fh_policy_bwd_bwd(void* stream, int dtype, int rows, int vocab, long long ld, const void* z,
                       const long long* actions, const float* stats, const float* g, const void* u, void* gz,
-                      float* gg);
+                      float* gg, float* scratch);
 
 /* Synchronises `stream`, then reads and clears the status word the kernels of
  * the current device record device-side failures in. *code receives 0 or one

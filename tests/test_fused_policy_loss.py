@@ -56,7 +56,7 @@ def _statement(z, a, old, adv, ref, w, lo=0.2, hi=0.2, beta=0.0, norm=None):
 
 CASES = [  # rows, vocab, ld, offset
     (1, 1, 1, 0), (1, 2, 2, 0), (3, 7, 9, 1), (5, 1000, 1000, 0), (4, 1001, 1001, 0), (6, 1003, 1008, 3),
-    (33, 4097, 4097, 0), (2, 131075, 131075, 0), (300, 513, 520, 0), (1, 40000, 40000, 5),
+    (33, 4097, 4097, 0), (2, 131075, 131075, 0), (40, 16391, 16400, 1), (130, 8192, 8192, 0), (300, 513, 520, 0), (1, 40000, 40000, 5),
 ]
 
 
@@ -309,4 +309,8 @@ def test_c_abi_refusals():
     assert fwd(old=None) == 1 and fwd(ref=None) == 1 and fwd(lo=-1.0) == 1 and fwd(norm=-1.0) == 1
     assert h.fh_policy_bwd(None, 0, 1, 4, 4, p, p, None, p, p) == 1
     assert h.fh_policy_bwd(None, 0, 0, 4, 4, p, p, p, p, p) == 0
-    assert h.fh_policy_bwd_bwd(None, 0, 1, 4, 4, p, p, p, p, None, p, p) == 1
+    assert h.fh_policy_bwd_bwd(None, 0, 1, 4, 4, p, p, p, p, None, p, p, None) == 1
+    assert h.fh_policy_bwd(None, 0, 1, 4, 4, p, p, ctypes.c_void_p(72), p, p) == 1  # stats not aligned
+    assert h.fh_policy_stats_floats(-1, 4) == -1 and h.fh_policy_scratch_floats(1, 0) == -1
+    assert h.fh_policy_scratch_floats(1, 100) == 0 and h.fh_policy_scratch_floats(1, 1 << 20) > 0
+    assert h.fh_policy_bwd_bwd(None, 0, 1, 1 << 20, 1 << 20, p, p, p, p, p, p, p, None) == 1  # needs scratch
