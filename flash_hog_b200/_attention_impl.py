@@ -127,11 +127,14 @@ def _is_f32(x: torch.Tensor, policy: str | None = None, mask=None) -> bool:
     return x.dtype == torch.float32 and (fp32_policy() if policy is None else policy) == "fp32"
 
 
+def _as(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return x if x.dtype is dtype else x.to(dtype)
+
+
 def _operand(x: torch.Tensor, f32: bool) -> torch.Tensor:
     """BTNH with a contiguous layout in the kernels' operand type (fp32 or bf16)."""
     dtype = torch.float32 if f32 else torch.bfloat16
-    if x.dtype is not dtype:
-        x = x.to(dtype)
+    x = _as(x, dtype)
     return x if x.is_contiguous() else x.contiguous()
 
 
@@ -178,8 +181,7 @@ def cuda_dot_product_attention(query, key, value, mask_type: MaskType, scale: fl
         _capi.attn_fwd_f32(q, k, v, out, lse, scale, *_mask_args(mask_type), **_mask_kw(mask_type))
     else:
         _capi.attn_fwd(q, k, v, out, lse, scale, *_mask_args(mask_type), **_mask_kw(mask_type))
-    if out.dtype is not query.dtype:
-        out = out.to(query.dtype)
+    out = _as(out, query.dtype)
     return (out, lse) if return_residual else out
 
 
@@ -209,7 +211,7 @@ def dot_product_attention_bwd_rule(mask_type: MaskType, scale: float, res, g, po
     else:
         _capi.attn_bwd(q, k, v, o, do, activation.float().contiguous(), dq, dk, dv, delta, scale,
                        *_mask_args(mask_type), **_mask_kw(mask_type))
-    return dq.to(query.dtype), dk.to(key.dtype), dv.to(value.dtype)
+    return _as(dq, query.dtype), _as(dk, key.dtype), _as(dv, value.dtype)
 
 
 def dot_product_attention_bwd_rule_fwd_rule(mask_type: MaskType, scale: float, res, g, policy: str | None = None):

@@ -174,7 +174,7 @@ def lib() -> ctypes.CDLL:
 
 
 def _check(entry: str, rc: int) -> None:
-    if rc != FH_OK:
+    if rc:
         detail = lib().fh_last_error().decode()
         msg = lib().fh_status_string(rc).decode() + (f": {detail}" if detail else "")
         raise FlashHogError(entry, rc, msg)
@@ -197,20 +197,32 @@ def _on_device(f):
 
     @functools.wraps(f)
     def call(t, *args, **kwargs):
-        if not t.is_cuda or t.get_device() == torch.cuda.current_device():
+        index = t.get_device()  # -1: not a CUDA tensor, which f refuses
+        if index < 0 or index == torch.cuda.current_device():
             return f(t, *args, **kwargs)
-        with torch.cuda.device(t.device):
+        with torch.cuda.device(index):
             return f(t, *args, **kwargs)
 
     return call
 
 
 def _same_device(t: torch.Tensor, *others) -> None:
-    if not t.is_cuda:
+    index = t.get_device()
+    if index < 0:
         raise ValueError("flash_hog_b200 runs on CUDA tensors only")
     for x in others:
-        if x is not None and x.device != t.device:
+        if x is not None and x.get_device() != index:
             raise ValueError(f"tensors must be on one CUDA device, got {t.device} and {x.device}")
+
+
+# Addresses and streams as plain integers, which ctypes converts by the argtypes: for the
+# small calls, whose time is the host's, building c_void_p objects is a tenth of it.
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _strides(t: torch.Tensor) -> FhStrides:
@@ -301,16 +313,16 @@ def attn_fwd(q, k, v, out, lse, scale: float, causal: int, window: int = 0, varl
     _same_layout(q, out)
     _same_layout(k, v)
     dims = make_dims(q, k, window, varlen, sinks)
-    _check("fh_attn_fwd", lib().fh_attn_fwd(_stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v),
-                                           _ptr(out), _ptr(lse), float(scale), int(causal)))
+    _check("fh_attn_fwd", lib().fh_attn_fwd(_raw_stream(q), ctypes.byref(dims), _addr(q), _addr(k), _addr(v),
+                                           _addr(out), _addr(lse), float(scale), int(causal)))
 
 
 @_on_device
 def attn_rowdot(o, dO, delta, varlen: Varlen | None = None) -> None:
     _same_layout(o, dO)
     dims = make_dims(o, o, 0, varlen)
-    _check("fh_attn_rowdot", lib().fh_attn_rowdot(_stream(o.device), ctypes.byref(dims), _ptr(o), _ptr(dO),
-                                                 _ptr(delta)))
+    _check("fh_attn_rowdot", lib().fh_attn_rowdot(_raw_stream(o), ctypes.byref(dims), _addr(o), _addr(dO),
+                                                 _addr(delta)))
 
 
 @_on_device
@@ -320,9 +332,9 @@ def attn_bwd(q, k, v, o, dO, lse, dq, dk, dv, delta, scale: float, causal: int, 
     _same_layout(k, v, dk, dv)
     dims = make_dims(q, k, window, varlen, sinks)
     scratch = _sink_scratch(dims, causal, q.device)  # noqa: F841 - held until the call is queued
-    _check("fh_attn_bwd", lib().fh_attn_bwd(_stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v),
-                                           _ptr(o), _ptr(dO), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv),
-                                           _ptr(delta), float(scale), int(causal)))
+    _check("fh_attn_bwd", lib().fh_attn_bwd(_raw_stream(q), ctypes.byref(dims), _addr(q), _addr(k), _addr(v),
+                                           _addr(o), _addr(dO), _addr(lse), _addr(dq), _addr(dk), _addr(dv),
+                                           _addr(delta), float(scale), int(causal)))
 
 
 @_on_device
@@ -334,8 +346,8 @@ def attn_bwdbwd(q, k, v, dO, ddq, ddk, ddv, lse, delta, dq2, ddo, dk2, dv2, dd, 
     dims = make_dims(q, k, window, varlen, sinks)
     scratch = _sink_scratch(dims, causal, q.device)  # noqa: F841 - held until the call is queued
     _check("fh_attn_bwdbwd", lib().fh_attn_bwdbwd(
-        _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(dO), _ptr(ddq), _ptr(ddk),
-        _ptr(ddv), _ptr(lse), _ptr(delta), _ptr(dq2), _ptr(ddo), _ptr(dk2), _ptr(dv2), _ptr(dd), _ptr(bvec),
+        _raw_stream(q), ctypes.byref(dims), _addr(q), _addr(k), _addr(v), _addr(dO), _addr(ddq), _addr(ddk),
+        _addr(ddv), _addr(lse), _addr(delta), _addr(dq2), _addr(ddo), _addr(dk2), _addr(dv2), _addr(dd), _addr(bvec),
         float(scale), int(causal)))
 
 
@@ -352,8 +364,8 @@ def attn_bwdbwd_pass(q, k, v, dO, ddq, ddk, ddv, lse, delta, dq2, ddo, dk2, dv2,
     dims = make_dims(q, k, window, varlen, sinks)
     scratch = _sink_scratch(dims, causal, q.device)  # noqa: F841 - held until the call is queued
     _check("fh_attn_bwdbwd_pass", lib().fh_attn_bwdbwd_pass(
-        _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(dO), _ptr(ddq), _ptr(ddk),
-        _ptr(ddv), _ptr(lse), _ptr(delta), _ptr(dq2), _ptr(ddo), _ptr(dk2), _ptr(dv2), _ptr(dd), _ptr(bvec),
+        _raw_stream(q), ctypes.byref(dims), _addr(q), _addr(k), _addr(v), _addr(dO), _addr(ddq), _addr(ddk),
+        _addr(ddv), _addr(lse), _addr(delta), _addr(dq2), _addr(ddo), _addr(dk2), _addr(dv2), _addr(dd), _addr(bvec),
         float(scale), int(causal), int(which)))
 
 
@@ -367,9 +379,9 @@ def attn_bwdbwd_o(q, k, v, o, dO, ddq, ddk, ddv, lse, dq2, ddo, dk2, dv2, delta,
     dims = make_dims(q, k, window, varlen, sinks)
     scratch = _sink_scratch(dims, causal, q.device)  # noqa: F841 - held until the call is queued
     _check("fh_attn_bwdbwd_o", lib().fh_attn_bwdbwd_o(
-        _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dO), _ptr(ddq),
-        _ptr(ddk), _ptr(ddv), _ptr(lse), _ptr(dq2), _ptr(ddo), _ptr(dk2), _ptr(dv2), _ptr(delta), _ptr(dd),
-        _ptr(bvec), float(scale), int(causal), int(which)))
+        _raw_stream(q), ctypes.byref(dims), _addr(q), _addr(k), _addr(v), _addr(o), _addr(dO), _addr(ddq),
+        _addr(ddk), _addr(ddv), _addr(lse), _addr(dq2), _addr(ddo), _addr(dk2), _addr(dv2), _addr(delta), _addr(dd),
+        _addr(bvec), float(scale), int(causal), int(which)))
 
 
 @_on_device
@@ -382,9 +394,9 @@ def attn_jvp_bwd(q, k, v, o, dO, lse, tq, tk, tv, tdO, tdq, tdk, tdv, to, delta,
     dims = make_dims(q, k, window, varlen, sinks)
     scratch = _sink_scratch(dims, causal, q.device)  # noqa: F841 - held until the call is queued
     _check("fh_attn_jvp_bwd", lib().fh_attn_jvp_bwd(
-        _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dO), _ptr(lse), _ptr(tq),
-        _ptr(tk), _ptr(tv), _ptr(tdO), _ptr(tdq), _ptr(tdk), _ptr(tdv), _ptr(to),
-        _ptr(delta), _ptr(dd), _ptr(bvec), float(scale), int(causal)))
+        _raw_stream(q), ctypes.byref(dims), _addr(q), _addr(k), _addr(v), _addr(o), _addr(dO), _addr(lse), _addr(tq),
+        _addr(tk), _addr(tv), _addr(tdO), _addr(tdq), _addr(tdk), _addr(tdv), _addr(to),
+        _addr(delta), _addr(dd), _addr(bvec), float(scale), int(causal)))
 
 
 _F32 = torch.float32
@@ -396,8 +408,8 @@ def attn_fwd_f32(q, k, v, out, lse, scale: float, causal: int, window: int = 0, 
     _same_layout(q, out, dtype=_F32)
     _same_layout(k, v, dtype=_F32)
     dims = make_dims(q, k, window, None, sinks)
-    _check("fh_attn_fwd_f32", lib().fh_attn_fwd_f32(_stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k),
-                                                   _ptr(v), _ptr(out), _ptr(lse), float(scale), int(causal)))
+    _check("fh_attn_fwd_f32", lib().fh_attn_fwd_f32(_raw_stream(q), ctypes.byref(dims), _addr(q), _addr(k),
+                                                   _addr(v), _addr(out), _addr(lse), float(scale), int(causal)))
 
 
 @_on_device
@@ -406,9 +418,9 @@ def attn_bwd_f32(q, k, v, o, dO, lse, dq, dk, dv, delta, scale: float, causal: i
     _same_layout(q, o, dO, dq, dtype=_F32)
     _same_layout(k, v, dk, dv, dtype=_F32)
     dims = make_dims(q, k, window, None, sinks)
-    _check("fh_attn_bwd_f32", lib().fh_attn_bwd_f32(_stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k),
-                                                   _ptr(v), _ptr(o), _ptr(dO), _ptr(lse), _ptr(dq), _ptr(dk),
-                                                   _ptr(dv), _ptr(delta), float(scale), int(causal)))
+    _check("fh_attn_bwd_f32", lib().fh_attn_bwd_f32(_raw_stream(q), ctypes.byref(dims), _addr(q), _addr(k),
+                                                   _addr(v), _addr(o), _addr(dO), _addr(lse), _addr(dq), _addr(dk),
+                                                   _addr(dv), _addr(delta), float(scale), int(causal)))
 
 
 @_on_device
@@ -419,9 +431,9 @@ def attn_bwdbwd_f32(q, k, v, o, dO, ddq, ddk, ddv, lse, dq2, ddo, dk2, dv2, delt
     _same_layout(k, v, ddk, ddv, dk2, dv2, dtype=_F32)
     dims = make_dims(q, k, window, None, sinks)
     _check("fh_attn_bwdbwd_f32", lib().fh_attn_bwdbwd_f32(
-        _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dO), _ptr(ddq),
-        _ptr(ddk), _ptr(ddv), _ptr(lse), _ptr(dq2), _ptr(ddo), _ptr(dk2), _ptr(dv2), _ptr(delta), _ptr(dd),
-        _ptr(bvec), float(scale), int(causal), int(which)))
+        _raw_stream(q), ctypes.byref(dims), _addr(q), _addr(k), _addr(v), _addr(o), _addr(dO), _addr(ddq),
+        _addr(ddk), _addr(ddv), _addr(lse), _addr(dq2), _addr(ddo), _addr(dk2), _addr(dv2), _addr(delta), _addr(dd),
+        _addr(bvec), float(scale), int(causal), int(which)))
 
 
 @_on_device
@@ -432,9 +444,9 @@ def attn_jvp_bwd_f32(q, k, v, o, dO, lse, tq, tk, tv, tdO, tdq, tdk, tdv, to, de
     _same_layout(k, v, tk, tv, tdk, tdv, dtype=_F32)
     dims = make_dims(q, k, window, None, sinks)
     _check("fh_attn_jvp_bwd_f32", lib().fh_attn_jvp_bwd_f32(
-        _stream(q.device), ctypes.byref(dims), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dO), _ptr(lse), _ptr(tq),
-        _ptr(tk), _ptr(tv), _ptr(tdO), _ptr(tdq), _ptr(tdk), _ptr(tdv), _ptr(to),
-        _ptr(delta), _ptr(dd), _ptr(bvec), float(scale), int(causal)))
+        _raw_stream(q), ctypes.byref(dims), _addr(q), _addr(k), _addr(v), _addr(o), _addr(dO), _addr(lse), _addr(tq),
+        _addr(tk), _addr(tv), _addr(tdO), _addr(tdq), _addr(tdk), _addr(tdv), _addr(to),
+        _addr(delta), _addr(dd), _addr(bvec), float(scale), int(causal)))
 
 
 def _ln_rows(x: torch.Tensor, cols: int) -> int:
@@ -544,7 +556,7 @@ def _embed_args(rows, table, tokens):
 def embed_fwd(w, tokens, scale: float, y) -> None:
     """y_i = scale w[t_i]; see fh_embed_fwd."""
     args = _embed_args(y, w, tokens)
-    _check("fh_embed_fwd", lib().fh_embed_fwd(_stream(w.device), *args, _ptr(w), _ptr(tokens), float(scale), _ptr(y)))
+    _check("fh_embed_fwd", lib().fh_embed_fwd(_raw_stream(w), *args, _addr(w), _addr(tokens), float(scale), _addr(y)))
 
 
 @_on_device
@@ -552,30 +564,31 @@ def embed_bwd(dy, tokens, scale: float, padding_idx: int, dw) -> None:
     """dw[v] = scale sum_{t_i = v} dy_i; see fh_embed_bwd."""
     args = _embed_args(dy, dw, tokens)
     scratch = torch.empty(int(lib().fh_embed_scratch_bytes(args[1], args[3])), dtype=torch.uint8, device=dw.device)
-    _check("fh_embed_bwd", lib().fh_embed_bwd(_stream(dw.device), *args, _ptr(dy), _ptr(tokens), float(scale),
-                                             int(padding_idx), _ptr(dw), _ptr(scratch)))
+    _check("fh_embed_bwd", lib().fh_embed_bwd(_raw_stream(dw), *args, _addr(dy), _addr(tokens), float(scale),
+                                             int(padding_idx), _addr(dw), _addr(scratch)))
 
 
 @_on_device
 def embed_bwd_bwd(ddw, tokens, scale: float, padding_idx: int, ddy) -> None:
     """ddy_i = scale ddw[t_i], 0 for padding; see fh_embed_bwd_bwd."""
     args = _embed_args(ddy, ddw, tokens)
-    _check("fh_embed_bwd_bwd", lib().fh_embed_bwd_bwd(_stream(ddw.device), *args, _ptr(ddw), _ptr(tokens),
-                                                     float(scale), int(padding_idx), _ptr(ddy)))
+    _check("fh_embed_bwd_bwd", lib().fh_embed_bwd_bwd(_raw_stream(ddw), *args, _addr(ddw), _addr(tokens),
+                                                     float(scale), int(padding_idx), _addr(ddy)))
 
 
 @_on_device
 def dropout(x, res, y, seed, subsequence: int, limit: int) -> None:
     """y = res + keep x / (1 - limit / 65536); see fh_dropout. ``res`` may be None."""
     _same_device(x, res, y, seed)
-    if seed.dtype != torch.int64 or seed.numel() != 1:
+    if seed.dtype is not torch.int64 or seed.numel() != 1:
         raise ValueError("the dropout seed is an int64 tensor of one element")
-    for t in (x, res, y):
-        if t is not None and (t.dtype not in _GELU_DTYPES or not t.is_contiguous() or t.shape != x.shape):
+    shape = x.shape
+    for t in (x, y) if res is None else (x, y, res):
+        if t.dtype not in _GELU_DTYPES or not t.is_contiguous() or t.shape != shape:
             raise ValueError("dropout tensors are contiguous fp32 or bf16 tensors of one shape")
     _check("fh_dropout", lib().fh_dropout(
-        _stream(x.device), x.numel(), _GELU_DTYPES[x.dtype], _ptr(x), 0 if res is None else _GELU_DTYPES[res.dtype],
-        _ptr(res), _GELU_DTYPES[y.dtype], _ptr(y), _ptr(seed), int(subsequence), int(limit)))
+        _raw_stream(x), x.numel(), _GELU_DTYPES[x.dtype], _addr(x), 0 if res is None else _GELU_DTYPES[res.dtype],
+        _addr(res), _GELU_DTYPES[y.dtype], _addr(y), _addr(seed), int(subsequence), int(limit)))
 
 
 def _policy_args(z, actions, *vectors):
@@ -603,8 +616,8 @@ def policy_fwd(z, actions, old, adv, ref, weights, clip_low: float, clip_high: f
     """Loss, log probabilities and the backward's statistics; see fh_policy_fwd."""
     args = _policy_args(z, actions, old, adv, ref, weights, lp)
     _check("fh_policy_fwd", lib().fh_policy_fwd(
-        _stream(z.device), *args, _ptr(z), _ptr(actions), _ptr(old), _ptr(adv), _ptr(ref), _ptr(weights),
-        float(clip_low), float(clip_high), float(kl_coef), float(normalizer), _ptr(lp), _ptr(loss), _ptr(stats)))
+        _raw_stream(z), *args, _addr(z), _addr(actions), _addr(old), _addr(adv), _addr(ref), _addr(weights),
+        float(clip_low), float(clip_high), float(kl_coef), float(normalizer), _addr(lp), _addr(loss), _addr(stats)))
 
 
 @_on_device
@@ -614,8 +627,8 @@ def policy_bwd(z, actions, stats, g, dz) -> None:
     _same_device(z, stats, g, dz)
     if dz.dtype != z.dtype or not dz.is_contiguous() or dz.shape != z.shape:
         raise ValueError("dz is a contiguous tensor of the logits' shape and dtype")
-    _check("fh_policy_bwd", lib().fh_policy_bwd(_stream(z.device), *args, _ptr(z), _ptr(actions), _ptr(stats),
-                                               _ptr(g), _ptr(dz)))
+    _check("fh_policy_bwd", lib().fh_policy_bwd(_raw_stream(z), *args, _addr(z), _addr(actions), _addr(stats),
+                                               _addr(g), _addr(dz)))
 
 
 @_on_device
@@ -628,8 +641,8 @@ def policy_bwd_bwd(z, actions, stats, g, u, gz, gg) -> None:
             raise ValueError("u and gz are contiguous tensors of the logits' shape and dtype")
     n = int(lib().fh_policy_scratch_floats(z.shape[0], z.shape[1]))
     scratch = torch.empty(n, dtype=torch.float32, device=z.device) if n else None
-    _check("fh_policy_bwd_bwd", lib().fh_policy_bwd_bwd(_stream(z.device), *args, _ptr(z), _ptr(actions), _ptr(stats),
-                                                       _ptr(g), _ptr(u), _ptr(gz), _ptr(gg), _ptr(scratch)))
+    _check("fh_policy_bwd_bwd", lib().fh_policy_bwd_bwd(_raw_stream(z), *args, _addr(z), _addr(actions), _addr(stats),
+                                                       _addr(g), _addr(u), _addr(gz), _addr(gg), _addr(scratch)))
 
 
 def launch_count() -> int:

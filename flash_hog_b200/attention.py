@@ -31,8 +31,6 @@ kernels run once, the rule the reference gives its double backward
 
 from __future__ import annotations
 
-import inspect
-
 import torch
 from torch.autograd import forward_ad
 
@@ -88,7 +86,7 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
         result = attn_impl.cuda_dot_product_attention(query, key, value, mask_type=mask_type, scale=float(scale),
                                                       policy=policy)
     else:
-        result, _ = _DotProductAttention.apply(query, key, value, mask_type, float(scale), policy)
+        result, _ = _function(_Plain, query, key, value).apply(query, key, value, mask_type, float(scale), policy)
     if unbatched:
         result = result.squeeze(0)
     return result
@@ -118,8 +116,8 @@ def dot_product_attention_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, 
         scale = query.shape[-1] ** -0.5
     mask = _mask_of(is_causal, causal_alignment, sliding_window_length, sink_tokens)
     packed = PackedSequences(mask, cu_seqlens_q, cu_seqlens_k, int(max_seqlen_q), int(max_seqlen_k))
-    result, _ = _DotProductAttention.apply(query.unsqueeze(0), key.unsqueeze(0), value.unsqueeze(0), packed,
-                                           float(scale), "bf16")
+    result, _ = _function(_Plain, query, key, value).apply(query.unsqueeze(0), key.unsqueeze(0), value.unsqueeze(0),
+                                                           packed, float(scale), "bf16")
     return result.squeeze(0)
 
 
@@ -128,20 +126,28 @@ def _no_packed_vmap(mask_type):
         raise NotImplementedError("packed variable-length batches are not vmapped: pack the sequences instead")
 
 
+def _transformed(*ts) -> bool:
+    """Whether forward-mode differentiation or a ``torch.func`` transform is at work on ``ts``."""
+    return forward_ad._current_level >= 0 or any(torch._C._functorch.is_functorch_wrapped_tensor(t) for t in ts)
+
+
 def _untracked(*ts) -> bool:
     """Whether no derivative of a call on ``ts`` will be asked for, and no transform is at
     work on them: the kernel is called without an autograd node (about 20 us of host time)."""
-    if forward_ad._current_level >= 0 or any(torch._C._functorch.is_functorch_wrapped_tensor(t) for t in ts):
-        return False
-    return not torch.is_grad_enabled() or not any(t.requires_grad for t in ts)
+    return not _transformed(*ts) and (not torch.is_grad_enabled() or not any(t.requires_grad for t in ts))
+
+
+def _function(plain, *ts):
+    """``plain`` (one of the two Functions at the end), or under a transform the Function
+    that it stands for, which has the transforms' rules."""
+    return plain.stands_for if _transformed(*ts) else plain
 
 
 def _plain_backward(g) -> bool:
     """Whether a backward runs for its values alone: no graph of it is being built, and no
     forward-mode or ``torch.func`` transform is differentiating or batching it. It then
     calls the rule itself instead of an autograd node (about 30 us of host time less)."""
-    return (not torch.is_grad_enabled() and forward_ad._current_level < 0
-            and not torch._C._functorch.is_functorch_wrapped_tensor(g))
+    return not torch.is_grad_enabled() and not _transformed(g)
 
 
 class _DotProductAttention(torch.autograd.Function):
@@ -174,8 +180,8 @@ class _DotProductAttention(torch.autograd.Function):
                 mask_type=ctx.mask_type, scale=ctx.scale, res=(query, key, value, activation, out), g=g,
                 policy=ctx.policy)
         else:
-            dq, dk, dv = _DotProductAttentionBwd.apply(query, key, value, activation, out, g, ctx.mask_type, ctx.scale,
-                                                       ctx.policy)
+            dq, dk, dv = _function(_PlainBwd, query, key, value, g).apply(query, key, value, activation, out, g,
+                                                                          ctx.mask_type, ctx.scale, ctx.policy)
         return dq, dk, dv, None, None, None
 
     @staticmethod
@@ -237,7 +243,19 @@ class _DotProductAttentionBwd(torch.autograd.Function):
         return tuple(attn_impl._unfold(x, size) for x in (dq, dk, dv)), (0, 0, 0)
 
 
-# torch binds the arguments of a Function with setup_context to forward's signature in
-# every call; kept on the function, it is not worked out again each time (25 us).
-for _f in (_DotProductAttention, _DotProductAttentionBwd):
-    _f.forward.__signature__ = inspect.signature(_f.forward)
+def _plain(cls):
+    """``cls`` for reverse mode alone: the same forward, residuals and backward without a
+    ``setup_context`` of torch's, which binds and unwraps the arguments in every call
+    (about 25 us of host time)."""
+
+    def forward(ctx, *args):
+        out = cls.forward(*args)
+        cls.setup_context(ctx, args, out)
+        return out
+
+    return type(cls.__name__ + "Plain", (torch.autograd.Function,),
+                {"forward": staticmethod(forward), "backward": staticmethod(cls.backward), "stands_for": cls})
+
+
+_Plain = _plain(_DotProductAttention)
+_PlainBwd = _plain(_DotProductAttentionBwd)

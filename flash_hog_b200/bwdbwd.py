@@ -22,7 +22,7 @@ import inspect
 import torch
 
 from flash_hog_b200 import _capi
-from flash_hog_b200._attention_impl import (MaskType, PackedSequences, _fold, _is_f32, _mask_args, _operand, _unfold,
+from flash_hog_b200._attention_impl import (MaskType, PackedSequences, _as, _fold, _is_f32, _mask_args, _operand, _unfold,
                                             _mask_kw, fp32_policy)
 
 
@@ -90,7 +90,7 @@ def _bwdbwd_device(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal: int, window: int, s
     entry = _capi.attn_bwdbwd_f32 if f32 else _capi.attn_bwdbwd_o
     entry(q, k, v, o, do, ddq, ddk, ddv, lse, dq2, ddo, dk2, dv2, delta, dd, bvec, scale, causal, window=window,
           **{**_mask_kw(packed), "sinks": sinks})
-    return dq2.to(Q.dtype), dk2.to(K.dtype), dv2.to(V.dtype), ddo.to(dO.dtype), stats
+    return _as(dq2, Q.dtype), _as(dk2, K.dtype), _as(dv2, V.dtype), _as(ddo, dO.dtype), stats
 
 
 class _FlashBwdBwd(torch.autograd.Function):

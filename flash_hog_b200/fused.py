@@ -336,9 +336,16 @@ def dropout(x, p: float, seed, *, subsequence: int = 0, residual=None):
                dtype)
 
 
+def _f32(t):
+    """``t`` as a contiguous fp32 constant."""
+    if t.requires_grad:
+        t = t.detach()
+    return _contig(t if t.dtype is torch.float32 else t.float())
+
+
 def _policy_bwd_run(z, actions, stats, g):
     dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-    _capi.policy_bwd(z, actions, stats, g.detach().float().reshape(1), dz)
+    _capi.policy_bwd(z, actions, stats, _f32(g), dz)
     return dz
 
 
@@ -347,8 +354,8 @@ class _PolicyLossBwd(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, z, actions, stats, g):
-        g32 = g.detach().float().reshape(1)
-        dz = _policy_bwd_run(z, actions, stats, g)
+        g32 = _f32(g)
+        dz = _policy_bwd_run(z, actions, stats, g32)
         ctx.save_for_backward(z, actions, stats, g32)
         ctx.g_shape, ctx.g_dtype = g.shape, g.dtype
         return dz
@@ -411,10 +418,10 @@ def policy_loss(logits, actions, old_logprobs, advantages, *, ref_logprobs=None,
         raise ValueError("normalizer must be positive and finite")
     if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
         logits = logits.contiguous()
-    vec = lambda t: None if t is None else _contig(t.detach().float())
-    return _PolicyLoss.apply(logits, _contig(actions.long()), vec(old_logprobs), vec(advantages),
-                             vec(ref_logprobs) if kl_coef > 0.0 else None, vec(weights), float(clip_low),
-                             float(clip_high), float(kl_coef), 0.0 if normalizer is None else float(normalizer))
+    return _PolicyLoss.apply(logits, _contig(actions.long()), _f32(old_logprobs), _f32(advantages),
+                             _f32(ref_logprobs) if kl_coef > 0.0 else None, None if weights is None else _f32(weights),
+                             float(clip_low), float(clip_high), float(kl_coef),
+                             0.0 if normalizer is None else float(normalizer))
 
 
 class _SumOfSquares(torch.autograd.Function):
