@@ -11,8 +11,9 @@ backward runs on this package's kernels through ``dot_product_attention`` (two
 nested autograd Functions, the analogue of the reference's nested custom_vjp).
 With ``fused=True`` (the default for the "flash" model) LayerNorm, the MLP's GELU
 and the cross-entropy loss run on the fused kernels of ``flash_hog_b200.fused`` --
-forward, backward and double backward one kernel each -- and the MLP's contractions
-on cuBLAS (plain GEMMs); the embeddings stay in torch autograd. Data
+forward, backward and double backward one kernel each -- as do the embeddings, dropout
+with the residual additions and, for ``policy_objective``, the clipped policy loss; the
+MLP's contractions run on cuBLAS (plain GEMMs). Data
 parallelism: each rank computes the full step on its own token batch and the
 parameter gradients (penalty terms included) are averaged with one NCCL
 all-reduce over a flat buffer.
@@ -44,14 +45,22 @@ class GPTConfig:
     d_mlp: int = 3072
     vocab: int = 32000
     seq_len: int = 1024
+    dropout: float = 0.0       # after the embeddings and on both residual branches, in training mode
+    embed_scale: float = 1.0   # factor on the token embeddings
+    window: int | None = None  # sliding-window length of the attention (None: all earlier tokens)
+    sinks: int = 0             # first tokens that stay visible behind the window
 
 
-def naive_attention(q, k, v, is_causal=True):
+def naive_attention(q, k, v, is_causal=True, sliding_window_length=None, sink_tokens=0):
     """softmax(q k^T / sqrt(D) + causal mask) v in torch ops (BTNH), for reference runs."""
     scale = q.shape[-1] ** -0.5
     s = torch.einsum("bqhd,bkhd->bhqk", q.float(), k.float()) * scale
     if is_causal:
         keep = torch.ones(q.shape[1], k.shape[1], dtype=torch.bool, device=q.device).tril()
+        if sliding_window_length is not None:
+            far = torch.ones_like(keep).tril(-sliding_window_length)
+            far[:, :sink_tokens] = False
+            keep &= ~far
         s = s.masked_fill(~keep, float("-inf"))
     p = torch.softmax(s, dim=-1)
     return torch.einsum("bhqk,bkhd->bqhd", p, v.float()).to(q.dtype)
@@ -61,7 +70,8 @@ class Block(nn.Module):
     def __init__(self, cfg: GPTConfig, attention, fused: bool):
         super().__init__()
         ln = fused_ops.LayerNorm if fused else nn.LayerNorm
-        self.cfg, self.attention = cfg, attention
+        self.cfg, self.attention, self.fused = cfg, attention, fused
+        self.mask = {} if cfg.window is None else dict(sliding_window_length=cfg.window, sink_tokens=cfg.sinks)
         self.act = fused_ops.gelu if fused else F.gelu
         self.ln1 = ln(cfg.d_model)
         self.qkv = nn.Linear(cfg.d_model, 3 * cfg.d_model)
@@ -70,28 +80,49 @@ class Block(nn.Module):
         self.fc1 = nn.Linear(cfg.d_model, cfg.d_mlp)
         self.fc2 = nn.Linear(cfg.d_mlp, cfg.d_model)
 
-    def forward(self, x):
+    def _add(self, x, branch, seed, subsequence):
+        """x + dropout(branch); ``seed`` None: without dropout."""
+        if seed is None:
+            return x + branch
+        if self.fused:
+            return fused_ops.dropout(branch, self.cfg.dropout, seed, subsequence=subsequence, residual=x)
+        return x + F.dropout(branch, self.cfg.dropout)
+
+    def forward(self, x, seed=None, index=0):
         b, t, d = x.shape
         h = self.cfg.n_head
         # One projection, then one copy to (3, b, t, h, dh): q, k and v come out contiguous,
         # so the attention op (and its backward and double backward) copies none of them.
         qkv = self.qkv(self.ln1(x)).view(b, t, 3, h, d // h).permute(2, 0, 1, 3, 4).contiguous()
         q, k, v = qkv.unbind(0)
-        x = x + self.proj(self.attention(q, k, v, is_causal=True).reshape(b, t, d))
-        return x + self.fc2(self.act(self.fc1(self.ln2(x))))
+        attn = self.attention(q, k, v, is_causal=True, **self.mask).reshape(b, t, d)
+        x = self._add(x, self.proj(attn), seed, 2 * index + 1)
+        return self._add(x, self.fc2(self.act(self.fc1(self.ln2(x)))), seed, 2 * index + 2)
 
 
 class GPT(nn.Module):
     """Pre-LN GPT; ``attention`` is "flash" (the sm_100a op) or "naive" (torch math);
-    ``fused`` (default: with "flash") puts LayerNorm and GELU on the fused kernels."""
+    ``fused`` (default: with "flash") puts the embeddings, LayerNorm, GELU and dropout on
+    the fused kernels.
+
+    With ``cfg.dropout`` each forward in training mode takes the next seed of the buffer
+    ``dropout_seed`` (an int64 tensor of one element, from 0; give data-parallel ranks
+    different starts): the masks of a step are a function of it, and steps replayed as a
+    CUDA graph advance it too."""
 
     def __init__(self, cfg: GPTConfig, attention: str = "flash", fused: bool | None = None):
         super().__init__()
         fn = {"flash": dot_product_attention, "naive": naive_attention}[attention]
         fused = attention == "flash" if fused is None else fused
         self.cfg, self.fused = cfg, fused
-        self.wte = nn.Embedding(cfg.vocab, cfg.d_model)
-        self.wpe = nn.Embedding(cfg.seq_len, cfg.d_model)
+        if fused:
+            self.wte = fused_ops.Embedding(cfg.vocab, cfg.d_model, scale=cfg.embed_scale)
+            self.wpe = fused_ops.Embedding(cfg.seq_len, cfg.d_model)
+        else:
+            self.wte = nn.Embedding(cfg.vocab, cfg.d_model)
+            self.wpe = nn.Embedding(cfg.seq_len, cfg.d_model)
+        if cfg.dropout > 0:
+            self.register_buffer("dropout_seed", torch.zeros(1, dtype=torch.long), persistent=False)
         self.blocks = nn.ModuleList(Block(cfg, fn, fused) for _ in range(cfg.n_layer))
         self.ln_f = (fused_ops.LayerNorm if fused else nn.LayerNorm)(cfg.d_model)
         self.apply(self._init)
@@ -108,9 +139,17 @@ class GPT(nn.Module):
 
     def forward(self, tokens):
         t = tokens.shape[1]
-        x = self.wte(tokens) + self.wpe(torch.arange(t, device=tokens.device))
-        for blk in self.blocks:
-            x = blk(x)
+        x = self.wte(tokens)
+        if not self.fused and self.cfg.embed_scale != 1.0:
+            x = x * self.cfg.embed_scale
+        x = x + self.wpe(torch.arange(t, device=tokens.device))
+        seed = None
+        if self.training and self.cfg.dropout > 0:
+            seed = self.dropout_seed.clone()  # the backward passes draw the masks of this step again
+            self.dropout_seed += 1
+            x = fused_ops.dropout(x, self.cfg.dropout, seed) if self.fused else F.dropout(x, self.cfg.dropout)
+        for i, blk in enumerate(self.blocks):
+            x = blk(x, seed, i)
         return self.ln_f(x) @ self.wte.weight.t()  # tied LM head
 
 
@@ -129,6 +168,23 @@ def penalty_objective(model: GPT, tokens: torch.Tensor, lam: float):
     else:
         penalty = sum((g.float() ** 2).sum() for g in grads)
     return loss + lam * penalty, loss.detach(), penalty.detach()
+
+
+def policy_objective(model: GPT, tokens: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor,
+                     lam: float = 0.0, **kwargs):
+    """(L + lam ||dL/dtheta||^2, L, log probabilities) for the clipped policy loss L of the
+    tokens' own successors: ``tokens`` (B, T+1), everything else (B, T) over the T
+    predictions (``weights`` of 0 for prompt and padding). ``kwargs`` are those of
+    ``fused.policy_loss``. With ``lam`` 0 no gradient is taken here."""
+    b, t = tokens.shape[0], tokens.shape[1] - 1
+    rows = {n: v.reshape(b * t) if isinstance(v, torch.Tensor) else v for n, v in kwargs.items()}
+    loss, logprobs = fused_ops.policy_loss(model(tokens[:, :-1]).flatten(0, 1), tokens[:, 1:].reshape(b * t),
+                                           old_logprobs.reshape(b * t), advantages.reshape(b * t), **rows)
+    total = loss
+    if lam:
+        grads = torch.autograd.grad(loss, [p for p in model.parameters() if p.requires_grad], create_graph=True)
+        total = loss + lam * fused_ops.sum_of_squares(grads)
+    return total, loss.detach(), logprobs.view(b, t)
 
 
 def allreduce_grads(model: nn.Module, group=None) -> None:
@@ -227,6 +283,23 @@ class PenaltyStepGraph:
         if optimizer is not None:
             optimizer.step()
         return self.loss, self.penalty
+
+
+def policy_step(model: GPT, tokens: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor,
+                lam: float = 0.0, optimizer=None, distributed: bool = False, autocast: bool = True, **kwargs):
+    """One step on ``policy_objective``: its gradient, the data-parallel gradient average and
+    the optimizer update. Returns (loss, log probabilities of the tokens (B, T))."""
+    with torch.autocast(device_type=tokens.device.type, dtype=torch.bfloat16,
+                        enabled=autocast and tokens.device.type == "cuda"):
+        total, loss, logprobs = policy_objective(model, tokens, old_logprobs, advantages, lam, **kwargs)
+    if optimizer is not None:
+        optimizer.zero_grad(set_to_none=True)
+    total.backward()
+    if distributed:
+        allreduce_grads(model)
+    if optimizer is not None:
+        optimizer.step()
+    return loss, logprobs
 
 
 def train_step(model: GPT, tokens: torch.Tensor, lam: float, optimizer=None, distributed: bool = False,
