@@ -32,7 +32,6 @@ kernels run once, the rule the reference gives its double backward
 from __future__ import annotations
 
 import torch
-from torch.autograd import forward_ad
 
 from flash_hog_b200 import _attention_impl as attn_impl
 from flash_hog_b200._attention_impl import MaskType, PackedSequences, SlidingWindow
@@ -82,7 +81,7 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
     # The fp32 policy is decided once here and kept with the residuals: the backward,
     # double backward and forward-mode rules of this graph all follow it.
     policy = attn_impl.fp32_policy()
-    if _untracked(query, key, value):
+    if attn_impl.untracked(query, key, value):
         result = attn_impl.cuda_dot_product_attention(query, key, value, mask_type=mask_type, scale=float(scale),
                                                       policy=policy)
     else:
@@ -126,28 +125,17 @@ def _no_packed_vmap(mask_type):
         raise NotImplementedError("packed variable-length batches are not vmapped: pack the sequences instead")
 
 
-def _transformed(*ts) -> bool:
-    """Whether forward-mode differentiation or a ``torch.func`` transform is at work on ``ts``."""
-    return forward_ad._current_level >= 0 or any(torch._C._functorch.is_functorch_wrapped_tensor(t) for t in ts)
-
-
-def _untracked(*ts) -> bool:
-    """Whether no derivative of a call on ``ts`` will be asked for, and no transform is at
-    work on them: the kernel is called without an autograd node (about 20 us of host time)."""
-    return not _transformed(*ts) and (not torch.is_grad_enabled() or not any(t.requires_grad for t in ts))
-
-
 def _function(plain, *ts):
     """``plain`` (one of the two Functions at the end), or under a transform the Function
     that it stands for, which has the transforms' rules."""
-    return plain.stands_for if _transformed(*ts) else plain
+    return plain.stands_for if attn_impl.transformed(*ts) else plain
 
 
 def _plain_backward(g) -> bool:
     """Whether a backward runs for its values alone: no graph of it is being built, and no
     forward-mode or ``torch.func`` transform is differentiating or batching it. It then
     calls the rule itself instead of an autograd node (about 30 us of host time less)."""
-    return not torch.is_grad_enabled() and not _transformed(g)
+    return not torch.is_grad_enabled() and not attn_impl.transformed(g)
 
 
 class _DotProductAttention(torch.autograd.Function):

@@ -22,8 +22,8 @@ import inspect
 import torch
 
 from flash_hog_b200 import _capi
-from flash_hog_b200._attention_impl import (MaskType, PackedSequences, _as, _fold, _is_f32, _mask_args, _operand, _unfold,
-                                            _mask_kw, fp32_policy)
+from flash_hog_b200._attention_impl import (MaskType, PackedSequences, _as, _fold, _is_f32, _mask_args, _mask_kw,
+                                            _operand, _unfold, fp32_policy, untracked)
 
 
 @dataclasses.dataclass(frozen=True)
@@ -66,8 +66,9 @@ def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, mask_type: MaskType = MaskTyp
     causal, window = _mask_args(mask_type)
     policy = fp32_policy() if _policy is None else _policy
     packed = mask_type if isinstance(mask_type, PackedSequences) else None
-    dq2, dk2, dv2, ddo, stats = _FlashBwdBwd.apply(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal, window, float(scale),
-                                                   policy, packed, _mask_kw(mask_type).get("sinks", 0))
+    run = _bwdbwd if untracked(Q, K, V, O, dO, ddQ, ddK, ddV, L) else _FlashBwdBwd.apply
+    dq2, dk2, dv2, ddo, stats = run(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal, window, float(scale), policy, packed,
+                                    _mask_kw(mask_type).get("sinks", 0))
     outs = (dq2, dk2, dv2, ddo)
     if return_stats:
         return outs, (stats[0], stats[1], stats[2])
@@ -93,6 +94,11 @@ def _bwdbwd_device(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal: int, window: int, s
     return _as(dq2, Q.dtype), _as(dk2, K.dtype), _as(dv2, V.dtype), _as(ddo, dO.dtype), stats
 
 
+def _bwdbwd(*args):
+    """``_bwdbwd_device``, its ``sinks`` (the last argument) given where there are any."""
+    return _bwdbwd_device(*args[:-1], **({"sinks": args[-1]} if args[-1] else {}))
+
+
 class _FlashBwdBwd(torch.autograd.Function):
     """The double backward as an autograd Function, so that ``torch.func`` transforms
     reach its batching rule instead of handing batched wrappers to the C ABI.
@@ -100,8 +106,7 @@ class _FlashBwdBwd(torch.autograd.Function):
 
     @staticmethod
     def forward(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal, window, scale, policy, packed, sinks):
-        return _bwdbwd_device(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal, window, scale, policy, packed,
-                              **({"sinks": sinks} if sinks else {}))
+        return _bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal, window, scale, policy, packed, sinks)
 
     @staticmethod
     def setup_context(ctx, inputs, output):

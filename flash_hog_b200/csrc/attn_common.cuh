@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "tc05.cuh"
 
@@ -64,10 +65,21 @@ struct AttnShape {
   const int* cu_q;            // varlen sequence starts (B + 1 entries), or null (dense)
   const int* cu_k;
   int total_q, total_k;       // rows of the packed tensors (varlen); Tq, Tk (dense)
-  int sinks;                  // first keys that a window leaves visible (0 without a window)
-  int splits;                 // parts the key passes cut a sink tile's queries into (sink_splits)
-  float* sink_part;           // splits > 1: their fp32 partial sums (sink_part_floats)
 };
+
+// A problem with sinks. A type of its own, for kernels of their own (SNK): three more
+// members in the others' parameters change their register allocation (the fp32 kernels ran
+// 1.5% slower).
+struct SinkShape : AttnShape {
+  int sinks;         // first keys that a window leaves visible (0 without a window)
+  int splits;        // parts the key passes cut a sink tile's queries into (sink_splits)
+  float* sink_part;  // splits > 1: their fp32 partial sums (sink_part_floats)
+};
+template <bool SNK>
+using ShapeOf = typename std::conditional<SNK, SinkShape, AttnShape>::type;
+
+__host__ __device__ __forceinline__ int sinks_of(const AttnShape&) { return 0; }
+__host__ __device__ __forceinline__ int sinks_of(const SinkShape& s) { return s.sinks; }
 
 // Where sequence b's rows start: the batch coordinate of its tensors' views and
 // its first query and key row (0, 0 for a dense batch).
@@ -80,13 +92,13 @@ struct SeqRange {
 // inconsistent cu_seqlens never address a row outside them.
 // Kernels are instantiated for dense (VL = false: `s` itself, no varlen arithmetic)
 // and packed (VL = true) batches.
-template <bool VL>
-__device__ __forceinline__ AttnShape seq_shape(const AttnShape& s, int b, SeqRange* r) {
+template <bool VL, class Shape>
+__device__ __forceinline__ Shape seq_shape(const Shape& s, int b, SeqRange* r) {
   if constexpr (!VL) {
     *r = SeqRange{b, 0, 0};
     return s;
   }
-  AttnShape l = s;
+  Shape l = s;
   const int q0 = max(0, min(s.cu_q[b], s.total_q)), q1 = max(q0, min(s.cu_q[b + 1], s.total_q));
   const int k0 = max(0, min(s.cu_k[b], s.total_k)), k1 = max(k0, min(s.cu_k[b + 1], s.total_k));
   l.Tq = min(q1 - q0, s.Tq);
@@ -108,7 +120,10 @@ __host__ __device__ __forceinline__ int query_lo(const AttnShape& s, int j) {
   return s.causal ? max(0, j - s.diag) : 0;
 }
 __host__ __device__ __forceinline__ int query_hi(const AttnShape& s, int j) {
-  return (s.causal && s.window > 0 && j >= s.sinks) ? min(s.Tq - 1, j - s.diag + s.window - 1) : s.Tq - 1;
+  return (s.causal && s.window > 0) ? min(s.Tq - 1, j - s.diag + s.window - 1) : s.Tq - 1;
+}
+__host__ __device__ __forceinline__ int query_hi(const SinkShape& s, int j) {
+  return j < s.sinks ? s.Tq - 1 : query_hi(static_cast<const AttnShape&>(s), j);
 }
 
 // Streamed tiles of `bn` rows that query rows [r0, r0 + rows) need: tiles
@@ -129,7 +144,7 @@ struct SinkTiles {
   int n, split, jump;  // from entry `split` on the window's tiles, `jump` further
   __host__ __device__ __forceinline__ int tile(int it) const { return it < split ? it : it + jump; }
 };
-__host__ __device__ __forceinline__ SinkTiles sink_key_tiles(const AttnShape& s, int r0, int rows, int bn) {
+__host__ __device__ __forceinline__ SinkTiles sink_key_tiles(const SinkShape& s, int r0, int rows, int bn) {
   SinkTiles t{0, 0, 0};
   const int r1 = min(r0 + rows, s.Tq) - 1;
   if (r1 < r0) return t;
@@ -149,12 +164,13 @@ __host__ __device__ __forceinline__ SinkTiles sink_key_tiles(const AttnShape& s,
 }
 
 // Streamed tiles of `bn` query rows that key rows [k0, k0 + rows) need.
-__host__ __device__ __forceinline__ int query_tiles(const AttnShape& s, int k0, int rows, int bn, int* first) {
+template <class Shape>
+__host__ __device__ __forceinline__ int query_tiles(const Shape& s, int k0, int rows, int bn, int* first) {
   const int k1 = min(k0 + rows, s.Tk) - 1;
   *first = 0;
   if (k1 < k0) return 0;
   // A tile that holds a sink is seen by every query from its first key's on.
-  const int lo = query_lo(s, k0), hi = k0 < s.sinks ? s.Tq - 1 : query_hi(s, k1);
+  const int lo = query_lo(s, k0), hi = query_hi(s, k0 < sinks_of(s) ? k0 : k1);
   if (hi < lo) return 0;
   *first = lo / bn;
   return hi / bn + 1 - *first;
@@ -187,7 +203,7 @@ inline int locality_group(int pairs, int shared, long long bytes_per_head) {
 }
 
 // Key tiles (of kBM keys) that hold a sink.
-__host__ __device__ __forceinline__ int sink_tiles(const AttnShape& s) {
+__host__ __device__ __forceinline__ int sink_tiles(const SinkShape& s) {
   return (min(s.sinks, s.Tk) + kBM - 1) / kBM;
 }
 
@@ -197,7 +213,7 @@ __host__ __device__ __forceinline__ int sink_tiles(const AttnShape& s) {
 // window 2048: dK/dV 476 us whole, 128 us in 4 parts and the join 3 us). As many parts as
 // make them about equal to ordinary tiles, but no more than it takes to fill the GPU a few
 // times over: each costs a partial sum of 2 x kBM x head_dim floats and a share of the join.
-inline int sink_splits(const AttnShape& s) {
+inline int sink_splits(const SinkShape& s) {
   const long long own = static_cast<long long>(s.window) + kBM + 64;
   if (s.sinks <= 0 || own >= s.Tq) return 1;
   const long long parts = (s.Tq + own - 1) / own;
@@ -210,28 +226,31 @@ inline int sink_splits(const AttnShape& s) {
 // with the join). The persistent key pass of the double backward deals its items out in
 // advance and wants equal ones (B4 H12 S1024 D64, window 256: 48 us
 // whole, 45 us in parts with the join; 120 and 119 us at the shape above).
-inline bool sink_whole(const AttnShape& s) {
+inline bool sink_whole(const SinkShape& s) {
   const long long own = static_cast<long long>(s.window) + kBM + 64;
   const long long ns = sink_tiles(s), nk = (s.Tk + kBM - 1) / kBM;
   return 4ll * s.Tq <= 3 * (static_cast<long long>(s.Hk) * s.B * ((nk - ns) * own + ns * s.Tq) / 148);
 }
-inline long long sink_part_floats(const AttnShape& s, int hd, int splits) {
+inline long long sink_part_floats(const SinkShape& s, int hd, int splits) {
   return splits > 1 ? 2ll * kBM * hd * splits * s.Hk * s.B * sink_tiles(s) : 0;
 }
 
+// How a key pass takes the sinks: there are none; their tiles whole; their tiles in parts.
+enum SinkMode : int { kNoSinks = 0, kSinksWhole = 1, kSinksSplit = 2 };
+
 // Work of a key pass with split sink tiles, in slots of (key tile, part): first the parts
 // of the sink tiles, then the ordinary tiles whole.
-__host__ __device__ __forceinline__ int split_slots(const AttnShape& s, int tiles) {
+__host__ __device__ __forceinline__ int split_slots(const SinkShape& s, int tiles) {
   return tiles + min(sink_tiles(s), tiles) * (s.splits - 1);
 }
 // Slot z's key tile; *part: which part of it, -1 = whole.
-__device__ __forceinline__ int split_slot(const AttnShape& s, int z, int* part) {
+__device__ __forceinline__ int split_slot(const SinkShape& s, int z, int* part) {
   const int cut = sink_tiles(s) * s.splits;
   *part = z < cut ? z % s.splits : -1;
   return z < cut ? z / s.splits : z - cut + cut / s.splits;
 }
 // Part p of the streamed tiles [0, total): *first and the number of them.
-__device__ __forceinline__ int split_range(const AttnShape& s, int total, int p, int* first) {
+__device__ __forceinline__ int split_range(const SinkShape& s, int total, int p, int* first) {
   if (p < 0) {
     *first = 0;
     return total;
@@ -241,7 +260,8 @@ __device__ __forceinline__ int split_range(const AttnShape& s, int total, int p,
 }
 // The partial sums of part p of key tile kt of pair hb = (batch, key head): two matrices
 // (dK then dV) of kBM rows.
-__device__ __forceinline__ float* sink_part_row(const AttnShape& s, int hd, int kt, int hb, int p, int matrix, int row) {
+__device__ __forceinline__ float* sink_part_row(const SinkShape& s, int hd, int kt, int hb, int p, int matrix,
+                                                int row) {
   const size_t slot = (static_cast<size_t>(kt) * s.Hk * s.B + hb) * s.splits + p;
   return s.sink_part + ((slot * 2 + matrix) * kBM + row) * hd;
 }

@@ -30,8 +30,9 @@
 namespace fh {
 namespace {
 
+template <bool SNK>
 struct BwdArgs {
-  AttnShape sh;
+  ShapeOf<SNK> sh;
   const float* lse;
   float* delta;  // D = rowsum(dO o O): written by the query-tiled pass, read by the key-tiled pass
   __nv_bfloat16* dq;
@@ -109,7 +110,7 @@ template <int HD, bool VL, bool GRP, bool SNK>
 __global__ void __launch_bounds__(kBBThreads, DqPass<HD>::CTAS)
     bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                   const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                  const __grid_constant__ CUtensorMap tm_o, const BwdArgs a) {
+                  const __grid_constant__ CUtensorMap tm_o, const BwdArgs<SNK> a) {
   using G = DqPass<HD>;
   constexpr int BN = G::BN, ST = G::ST;
   extern __shared__ uint8_t smem_raw[];
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(kBBThreads, DqPass<HD>::CTAS)
     h = hb % a.sh.H, b = hb / a.sh.H, qt = nq - 1 - qi;
   }
   SeqRange sr;
-  const AttnShape sh = seq_shape<VL>(a.sh, b, &sr);  // this sequence's lengths and mask; sr: where its rows start
+  const ShapeOf<SNK> sh = seq_shape<VL>(a.sh, b, &sr);  // this sequence's lengths and mask; sr: where its rows start
   const int q0 = qt * kBM;
   int j0;
   int n = 0;  // key tiles j0, j0 + 1, ... or, with sinks, sink.tile(0), ... (0: no row sees a key)
@@ -303,10 +304,10 @@ __global__ void __launch_bounds__(kBBThreads, DqPass<HD>::CTAS)
         reg_fence(vdp);
         warp_arrive(&bar_sc_empty[wg]);  // the tensor core may reuse this score buffer now
         const int kc = key_row(j);
-        const bool need_mask = kc + BN - 1 > khi || (kc < klo && (!SNK || kc + BN > sh.sinks));
+        const bool need_mask = kc + BN - 1 > khi || (kc < klo && (!SNK || kc + BN > sinks_of(sh)));
         uint32_t o_ds[BN / 2];
         if (need_mask)
-          dq_ops<BN, SNK ? 2 : 1>(vs, vdp, kc, klo, khi, sh.sinks, sc2, lg, dv, o_ds);
+          dq_ops<BN, SNK ? 2 : 1>(vs, vdp, kc, klo, khi, sinks_of(sh), sc2, lg, dv, o_ds);
         else
           dq_ops<BN, 0>(vs, vdp, kc, klo, khi, 0, sc2, lg, dv, o_ds);
         if (u > 0) ok = mbar_wait_warp(&bar_ops_empty[wg], (u - 1) & 1, &abort_flag);
@@ -333,10 +334,10 @@ __global__ void __launch_bounds__(kBBThreads, DqPass<HD>::CTAS)
         reg_fence(vdp);
         warp_arrive(&bar_sc_empty[0]);
         const int kc = key_row(j) + cb;  // first key of this thread's columns
-        const bool need_mask = kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sh.sinks));
+        const bool need_mask = kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sinks_of(sh)));
         uint32_t o_ds[CW / 2];
         if (need_mask)
-          dq_ops<CW, SNK ? 2 : 1>(vs, vdp, kc, klo, khi, sh.sinks, sc2, lg, dv, o_ds);
+          dq_ops<CW, SNK ? 2 : 1>(vs, vdp, kc, klo, khi, sinks_of(sh), sc2, lg, dv, o_ds);
         else
           dq_ops<CW, 0>(vs, vdp, kc, klo, khi, 0, sc2, lg, dv, o_ds);
         if (j > 0) ok = mbar_wait_warp(&bar_ops_empty[0], (j - 1) & 1, &abort_flag);
@@ -441,15 +442,16 @@ __device__ __forceinline__ void dkv_ops(const uint32_t (&vs)[CW], const uint32_t
   }
 }
 
-// SPLIT: key tiles that hold a sink are cut into parts (split_slot); a part leaves fp32
-// partial sums, which launch_sink_join adds up.
-template <int HD, bool VL, bool GRP, bool SPLIT>
+// kSinksSplit: key tiles that hold a sink are cut into parts (split_slot); a part leaves
+// fp32 partial sums, which launch_sink_join adds up.
+template <int HD, bool VL, bool GRP, SinkMode SINKS>
 __global__ void __launch_bounds__(kBBThreads, DkvPass<HD>::CTAS)
     bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                     const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
-                    const BwdArgs a) {
+                    const BwdArgs<SINKS != kNoSinks> a) {
   using G = DkvPass<HD>;
   constexpr int BN = G::BN, ST = G::ST, CW = G::CW;
+  constexpr bool SNK = SINKS != kNoSinks, SPLIT = SINKS == kSinksSplit;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = align1024(smem_raw);
   uint8_t* s_k = sm;
@@ -470,10 +472,10 @@ __global__ void __launch_bounds__(kBBThreads, DkvPass<HD>::CTAS)
     grouped_order(blockIdx.x, (a.sh.Tk + kBM - 1) / kBM, a.sh.Hk * a.sh.B, a.grp_k, &kt, &hb);
     hk = hb % a.sh.Hk, b = hb / a.sh.Hk;
   }
-  int part = -1;
+  int part = -1;  // SPLIT: which part of a sink tile, -1 = whole
   if constexpr (SPLIT) kt = split_slot(a.sh, blockIdx.z, &part);
   SeqRange sr;
-  const AttnShape sh = seq_shape<VL>(a.sh, b, &sr);
+  const ShapeOf<SNK> sh = seq_shape<VL>(a.sh, b, &sr);
   const int k0 = kt * kBM;
   int qt_begin;
   const int n = query_tiles(sh, k0, kBM, BN, &qt_begin);  // query tiles that see any of these keys
@@ -519,9 +521,10 @@ __global__ void __launch_bounds__(kBBThreads, DkvPass<HD>::CTAS)
       const size_t off = k_row(sh, sr, key < sh.Tk ? key : 0, hk);
       const __nv_bfloat16* add = wg == 0 ? a.dk_acc : a.dv_acc;
       __nv_bfloat16* dst = (wg == 0 ? a.dk : a.dv) + off;
-      if (SPLIT && part >= 0) {
-        zero_row_f32<HD>(sink_part_row(a.sh, HD, kt, b * sh.Hk + hk, part, wg, key - k0));
-      } else if (key < sh.Tk) {
+      if constexpr (SPLIT) {
+        if (part >= 0) zero_row_f32<HD>(sink_part_row(a.sh, HD, kt, b * sh.Hk + hk, part, wg, key - k0));
+      }
+      if (part < 0 && key < sh.Tk) {
         if (add) {  // the outputs are the addends
           for (int c = 0; c < HD; c += 8)
             reinterpret_cast<uint4*>(dst + c)[0] = reinterpret_cast<const uint4*>(add + off + c)[0];
@@ -739,11 +742,13 @@ __global__ void __launch_bounds__(kBBThreads, DkvPass<HD>::CTAS)
     if (ok) ok = mbar_wait_warp(&bar_acc, 0, &abort_flag);
     if (ok) {
       tc_fence_after();
-      if (SPLIT && part >= 0) {
-        tmem_row_to_f32<HD>(tmem, warp, wg == 0 ? G::C_DK : G::C_DV,
-                            sink_part_row(a.sh, HD, kt, b * sh.Hk + hk, part, wg, r), key_ok,
-                            wg == 0 ? sh.scale : 1.f);
-      } else {
+      if constexpr (SPLIT) {
+        if (part >= 0)
+          tmem_row_to_f32<HD>(tmem, warp, wg == 0 ? G::C_DK : G::C_DV,
+                              sink_part_row(a.sh, HD, kt, b * sh.Hk + hk, part, wg, r), key_ok,
+                              wg == 0 ? sh.scale : 1.f);
+      }
+      if (part < 0) {
         const size_t off = k_row(sh, sr, key_ok ? key : 0, hk);
         const __nv_bfloat16* add = wg == 0 ? a.dk_acc : a.dv_acc;
         tmem_row_to_global<HD>(tmem, warp, wg == 0 ? G::C_DK : G::C_DV, (wg == 0 ? a.dk : a.dv) + off, key_ok,
@@ -760,7 +765,7 @@ __global__ void __launch_bounds__(kBBThreads, DkvPass<HD>::CTAS)
 }
 
 template <int HD, bool VL>
-int launch_bwd_hd(const AttnShape& s, const BwdPtrs& p, int* status, cudaStream_t stream) {
+int launch_bwd_hd(const SinkShape& s, const BwdPtrs& p, int* status, cudaStream_t stream) {
   using GQ = DqPass<HD>;
   using GK = DkvPass<HD>;
   CUtensorMap mq[5], mk[4];
@@ -774,59 +779,62 @@ int launch_bwd_hd(const AttnShape& s, const BwdPtrs& p, int* status, cudaStream_
             make_seq_map(&mk[2], p.q, HD, s.total_q, s.H, map_batch(s), s.sq, GK::BN) &&
             make_seq_map(&mk[3], p.dO, HD, s.total_q, s.H, map_batch(s), s.sq, GK::BN);
   if (!ok) return kInvalidArgument;
-  BwdArgs args{s,
-               p.lse,
-               p.delta,
-               static_cast<__nv_bfloat16*>(p.dq),
-               static_cast<__nv_bfloat16*>(p.dk),
-               static_cast<__nv_bfloat16*>(p.dv),
-               static_cast<const __nv_bfloat16*>(p.dq_acc),
-               static_cast<const __nv_bfloat16*>(p.dk_acc),
-               static_cast<const __nv_bfloat16*>(p.dv_acc),
-               status,
-               // Shared streamed tiles per head: K and V of a key head (dQ pass); Q and
-               // dO of its query heads (dK/dV pass).
-               locality_group(s.H * s.B, s.H / s.Hk, 2ll * s.Tk * HD * 2),
-               locality_group(s.Hk * s.B, 1, 2ll * (s.H / s.Hk) * s.Tq * HD * 2)};
+  // Shared streamed tiles per head: K and V of a key head (dQ pass); Q and dO of its query
+  // heads (dK/dV pass).
+  const int grp_q = locality_group(s.H * s.B, s.H / s.Hk, 2ll * s.Tk * HD * 2);
+  const int grp_k = locality_group(s.Hk * s.B, 1, 2ll * (s.H / s.Hk) * s.Tq * HD * 2);
+  auto make_args = [&](auto snk) {
+    return BwdArgs<decltype(snk)::value>{s,
+                                         p.lse,
+                                         p.delta,
+                                         static_cast<__nv_bfloat16*>(p.dq),
+                                         static_cast<__nv_bfloat16*>(p.dk),
+                                         static_cast<__nv_bfloat16*>(p.dv),
+                                         static_cast<const __nv_bfloat16*>(p.dq_acc),
+                                         static_cast<const __nv_bfloat16*>(p.dk_acc),
+                                         static_cast<const __nv_bfloat16*>(p.dv_acc),
+                                         status,
+                                         grp_q,
+                                         grp_k};
+  };
   const int nq = (s.Tq + kBM - 1) / kBM, nk = (s.Tk + kBM - 1) / kBM;
-  auto launch_q = [&](auto* kernel, dim3 grid) {
+  auto launch_q = [&](auto* kernel, dim3 grid, const auto& args) {
     if (ensure_smem_limit(reinterpret_cast<const void*>(kernel), GQ::SMEM) != kOk) return kLaunchFailed;
     kernel<<<grid, kBBThreads, GQ::SMEM, stream>>>(mq[0], mq[1], mq[2], mq[3], mq[4], args);
     return static_cast<HostStatus>(after_launch());
   };
-  auto launch_k = [&](auto* kernel, dim3 grid) {
+  auto launch_k = [&](auto* kernel, dim3 grid, const auto& args) {
     if (ensure_smem_limit(reinterpret_cast<const void*>(kernel), GK::SMEM) != kOk) return kLaunchFailed;
     kernel<<<grid, kBBThreads, GK::SMEM, stream>>>(mk[0], mk[1], mk[2], mk[3], args);
     return static_cast<HostStatus>(after_launch());
   };
-  // The grouped kernels only where the groups split the pairs, and not with sinks: their
-  // query tiles share few of their keys.
   const dim3 grid_q(s.H, s.B, nq), grid_k(s.Hk, s.B, nk);
-  HostStatus rc = kOk;
-  bool done = false;
-  if constexpr (!VL) {
-    if (s.sinks == 0 && args.grp_q < s.H * s.B) {
-      rc = launch_q(&bwd_dq_kernel<HD, false, true, false>, dim3(s.H * s.B * nq));
-      done = true;
-    }
-  }
-  if (!done)
-    rc = s.sinks > 0 ? launch_q(&bwd_dq_kernel<HD, VL, false, true>, grid_q)
-                     : launch_q(&bwd_dq_kernel<HD, VL, false, false>, grid_q);
-  if (rc != kOk) return rc;
-  if (s.splits > 1 && !sink_whole(s)) {
-    rc = launch_k(&bwd_dkdv_kernel<HD, VL, false, true>, dim3(s.Hk, s.B, split_slots(s, nk)));
+  if (s.sinks > 0) {  // plain order: the query tiles share few of their keys
+    const auto args = make_args(std::true_type{});
+    HostStatus rc = launch_q(&bwd_dq_kernel<HD, VL, false, true>, grid_q, args);
+    if (rc != kOk) return rc;
+    if (s.splits == 1 || sink_whole(s)) return launch_k(&bwd_dkdv_kernel<HD, VL, false, kSinksWhole>, grid_k, args);
+    rc = launch_k(&bwd_dkdv_kernel<HD, VL, false, kSinksSplit>, dim3(s.Hk, s.B, split_slots(s, nk)), args);
     return rc != kOk ? rc : launch_sink_join(s, HD, p.dk, p.dv, p.dk_acc, p.dv_acc, stream);
   }
+  // The grouped kernels only where the groups split the pairs.
+  const auto args = make_args(std::false_type{});
   if constexpr (!VL) {
-    if (args.grp_k < s.Hk * s.B) return launch_k(&bwd_dkdv_kernel<HD, false, true, false>, dim3(s.Hk * s.B * nk));
+    const HostStatus rc = grp_q < s.H * s.B
+                              ? launch_q(&bwd_dq_kernel<HD, false, true, false>, dim3(s.H * s.B * nq), args)
+                              : launch_q(&bwd_dq_kernel<HD, false, false, false>, grid_q, args);
+    if (rc != kOk) return rc;
+    return grp_k < s.Hk * s.B ? launch_k(&bwd_dkdv_kernel<HD, false, true, kNoSinks>, dim3(s.Hk * s.B * nk), args)
+                              : launch_k(&bwd_dkdv_kernel<HD, false, false, kNoSinks>, grid_k, args);
+  } else {
+    const HostStatus rc = launch_q(&bwd_dq_kernel<HD, true, false, false>, grid_q, args);
+    return rc != kOk ? rc : launch_k(&bwd_dkdv_kernel<HD, true, false, kNoSinks>, grid_k, args);
   }
-  return launch_k(&bwd_dkdv_kernel<HD, VL, false, false>, grid_k);
 }
 
 }  // namespace
 
-int launch_bwd(const AttnShape& s, int hd, const BwdPtrs& p, int* status, cudaStream_t stream) {
+int launch_bwd(const SinkShape& s, int hd, const BwdPtrs& p, int* status, cudaStream_t stream) {
   if (hd == 64) return s.cu_q ? launch_bwd_hd<64, true>(s, p, status, stream) : launch_bwd_hd<64, false>(s, p, status, stream);
   if (hd == 128) return s.cu_q ? launch_bwd_hd<128, true>(s, p, status, stream) : launch_bwd_hd<128, false>(s, p, status, stream);
   return kUnsupported;

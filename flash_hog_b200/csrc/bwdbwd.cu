@@ -32,8 +32,9 @@
 namespace fh {
 namespace {
 
+template <bool SNK>
 struct BBArgs {
-  AttnShape sh;
+  ShapeOf<SNK> sh;
   const float* lse;
   const float* delta;  // D = rowsum(dO o): read by both passes
   float* delta_out;    // non-null: the query pass computes D from o and writes it here (= delta)
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
                     const __grid_constant__ CUtensorMap tm_ddq, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_ddk,
                     const __grid_constant__ CUtensorMap tm_ddv, const __grid_constant__ CUtensorMap tm_o,
-                    const BBArgs a) {
+                    const BBArgs<SNK> a) {
   using G = QPass<HD>;
   constexpr int BN = G::BN, ST = G::ST;
   extern __shared__ uint8_t smem_raw[];
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
     h = hb % a.sh.H, b = hb / a.sh.H, qt = nq - 1 - qi;
   }
   SeqRange sr;
-  const AttnShape sh = seq_shape<VL>(a.sh, b, &sr);  // this sequence's lengths and mask; sr: where its rows start
+  const ShapeOf<SNK> sh = seq_shape<VL>(a.sh, b, &sr);  // this sequence's lengths and mask; sr: where its rows start
   const int q0 = qt * kBM;
   int j0;
   int n = 0;  // key tiles per sweep: j0, j0 + 1, ... or, with sinks, sink.tile(0), ... (0: no row sees a key)
@@ -458,13 +459,13 @@ __global__ void __launch_bounds__(kBBThreads, 1)
         ok = load_scores(j, vs, vdds, vdp, vdpa);
         if (!ok) break;
         if constexpr (TJ) {
-          if (kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sh.sinks)))
-            q_stats_tj<CW, SNK ? 2 : 1>(vs, vdds, kc, klo, khi, sh.sinks, sc2, lg, pdD);
+          if (kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sinks_of(sh))))
+            q_stats_tj<CW, SNK ? 2 : 1>(vs, vdds, kc, klo, khi, sinks_of(sh), sc2, lg, pdD);
           else
             q_stats_tj<CW, 0>(vs, vdds, kc, klo, khi, 0, sc2, lg, pdD);
         } else {
-          if (kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sh.sinks)))
-            q_stats<CW, SNK ? 2 : 1>(vs, vdds, vdp, vdpa, kc, klo, khi, sh.sinks, sc2, lg, pdD, pr1, pr2, pr3);
+          if (kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sinks_of(sh))))
+            q_stats<CW, SNK ? 2 : 1>(vs, vdds, vdp, vdpa, kc, klo, khi, sinks_of(sh), sc2, lg, pdD, pr1, pr2, pr3);
           else
             q_stats<CW, 0>(vs, vdds, vdp, vdpa, kc, klo, khi, 0, sc2, lg, pdD, pr1, pr2, pr3);
         }
@@ -496,13 +497,13 @@ __global__ void __launch_bounds__(kBBThreads, 1)
       if (!ok) break;
       uint32_t o_ds[CW / 2], o_ds2[CW / 2], o_ddp[CW / 2], o_p[CW / 2];
       if constexpr (TJ) {
-        if (kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sh.sinks)))
-          q_ops_tj<CW, SNK ? 2 : 1>(vs, vdds, kc, klo, khi, sh.sinks, sc, sc2, lg, dD, o_ddp, o_p);
+        if (kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sinks_of(sh))))
+          q_ops_tj<CW, SNK ? 2 : 1>(vs, vdds, kc, klo, khi, sinks_of(sh), sc, sc2, lg, dD, o_ddp, o_p);
         else
           q_ops_tj<CW, 0>(vs, vdds, kc, klo, khi, 0, sc, sc2, lg, dD, o_ddp, o_p);
       } else {
-        if (kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sh.sinks)))
-          q_ops<CW, SNK ? 2 : 1>(vs, vdds, vdp, vdpa, kc, klo, khi, sh.sinks, sc, sc2, lg, dv, dD, cq, o_ds, o_ds2, o_ddp, o_p);
+        if (kc + CW - 1 > khi || (kc < klo && (!SNK || kc + CW > sinks_of(sh))))
+          q_ops<CW, SNK ? 2 : 1>(vs, vdds, vdp, vdpa, kc, klo, khi, sinks_of(sh), sc, sc2, lg, dv, dD, cq, o_ds, o_ds2, o_ddp, o_p);
         else
           q_ops<CW, 0>(vs, vdds, vdp, vdpa, kc, klo, khi, 0, sc, sc2, lg, dv, dD, cq, o_ds, o_ds2, o_ddp, o_p);
       }
@@ -630,18 +631,19 @@ __device__ __forceinline__ void k_ops(const uint32_t (&vs)[CW], const uint32_t (
 
 // A unit of key-pass work: one 128-row key tile of one (key head, batch).
 // `l` is the item's sequence (its lengths and mask), `r` where that sequence's rows start.
+template <bool SNK>
 struct KItem {
   int hk, b, k0, qt_begin, n, total;  // n query tiles per query head; total = n * G streamed tiles
-  int base, part;                     // SPLIT: a part of a sink tile streams `total` tiles from `base` on (-1: whole)
-  AttnShape l;
+  int base, part;                     // a part of a sink tile streams `total` tiles from `base` on (-1: whole)
+  ShapeOf<SNK> l;
   SeqRange r;
 };
 
 // Work item w in heaviest-first order (key tile 0 first: the most causal query
 // tiles), key heads fastest; GRP: in locality groups of g (key head, batch) pairs.
-// SPLIT: the parts of the sinks' tiles first (split_slot).
-template <bool VL, bool GRP, bool SPLIT>
-__device__ __forceinline__ KItem k_item(const AttnShape& sh, int w, int bn, int g) {
+// kSinksSplit: the parts of the sinks' tiles first (split_slot).
+template <bool VL, bool GRP, SinkMode SINKS>
+__device__ __forceinline__ KItem<SINKS != kNoSinks> k_item(const ShapeOf<SINKS != kNoSinks>& sh, int w, int bn, int g) {
   int kt, hb, part = -1;
   if constexpr (GRP) {
     grouped_order(w, (sh.Tk + kBM - 1) / kBM, sh.Hk * sh.B, g, &kt, &hb);
@@ -649,9 +651,9 @@ __device__ __forceinline__ KItem k_item(const AttnShape& sh, int w, int bn, int 
     const int per_kt = sh.Hk * sh.B;
     kt = w / per_kt;
     hb = w - kt * per_kt;
-    if constexpr (SPLIT) kt = split_slot(sh, kt, &part);
+    if constexpr (SINKS == kSinksSplit) kt = split_slot(sh, kt, &part);
   }
-  KItem it;
+  KItem<SINKS != kNoSinks> it;
   it.hk = hb % sh.Hk;
   it.b = hb / sh.Hk;
   it.k0 = kt * kBM;
@@ -660,7 +662,7 @@ __device__ __forceinline__ KItem k_item(const AttnShape& sh, int w, int bn, int 
   it.total = it.n * sh.G;
   it.base = 0;
   it.part = part;
-  if constexpr (SPLIT) it.total = split_range(sh, it.total, part, &it.base);
+  if constexpr (SINKS == kSinksSplit) it.total = split_range(sh, it.total, part, &it.base);
   return it;
 }
 
@@ -671,14 +673,16 @@ __device__ __forceinline__ KItem k_item(const AttnShape& sh, int w, int bn, int 
 // MMAs of the previous item are done (bar_res_empty), so the reload overlaps the
 // previous item's last tile and epilogue, and the operand MMAs of an item start
 // only once the previous item's accumulators were read out (bar_acc_empty).
-template <int HD, bool VL, bool GRP, bool SPLIT>
+template <int HD, bool VL, bool GRP, SinkMode SINKS>
 __global__ void __launch_bounds__(kBBThreads, 1)
     bwdbwd_k_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                     const __grid_constant__ CUtensorMap tm_ddk, const __grid_constant__ CUtensorMap tm_ddv,
                     const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
-                    const __grid_constant__ CUtensorMap tm_ddq, const BBArgs a) {
+                    const __grid_constant__ CUtensorMap tm_ddq, const BBArgs<SINKS != kNoSinks> a) {
   using G = KPass<HD>;
   constexpr int BN = G::BN, ST = G::ST;
+  constexpr bool SPLIT = SINKS == kSinksSplit;
+  using Item = KItem<SINKS != kNoSinks>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = align1024(smem_raw);
   uint8_t* s_k = sm;
@@ -692,14 +696,16 @@ __global__ void __launch_bounds__(kBBThreads, 1)
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
 
-  const AttnShape& sh = a.sh;
+  const ShapeOf<SINKS != kNoSinks>& sh = a.sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int key_tiles_all = (sh.Tk + kBM - 1) / kBM;
-  const int n_items = sh.Hk * sh.B * (SPLIT ? split_slots(sh, key_tiles_all) : key_tiles_all);
+  int slots = key_tiles_all;
+  if constexpr (SPLIT) slots = split_slots(sh, key_tiles_all);
+  const int n_items = sh.Hk * sh.B * slots;
   const int P = gridDim.x, c = blockIdx.x;
   // First query and query head of streamed tile `it` of item `w`.
-  auto tile_q = [&](const KItem& w, int it) { return (w.qt_begin + (SPLIT ? w.base + it : it) % w.n) * BN; };
-  auto tile_h = [&](const KItem& w, int it) { return w.hk * sh.G + (SPLIT ? w.base + it : it) / w.n; };
+  auto tile_q = [&](const Item& w, int it) { return (w.qt_begin + (SPLIT ? w.base + it : it) % w.n) * BN; };
+  auto tile_h = [&](const Item& w, int it) { return w.hk * sh.G + (SPLIT ? w.base + it : it) / w.n; };
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -740,7 +746,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
     const float inv_scale = 1.f / sh.scale;
     constexpr int RPL = BN / 32;
     // Per-query statistics of streamed tile `it` of item `w`, into registers.
-    auto load_stats = [&](const KItem& w, int it, float (&raw)[RPL][4]) {
+    auto load_stats = [&](const Item& w, int it, float (&raw)[RPL][4]) {
       const int q0 = tile_q(w, it);
       const int h = tile_h(w, it);
 #pragma unroll
@@ -758,7 +764,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
     for (int j = 0; ok; ++j) {
       const int wi = snake_item(j, c, P);
       if (wi >= n_items) break;
-      const KItem w = k_item<VL, GRP, SPLIT>(sh, wi, BN, a.grp_k);
+      const Item w = k_item<VL, GRP, SINKS>(sh, wi, BN, a.grp_k);
       if (w.total == 0) continue;
       // The previous item's score MMAs no longer read the resident tiles.
       if (ai > 0 && !mbar_wait_warp(&bar_res_empty, (ai - 1) & 1, &abort_flag)) {
@@ -842,7 +848,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
     for (int j = 0; ok; ++j) {
       const int wi = snake_item(j, c, P);
       if (wi >= n_items) break;
-      const KItem w = k_item<VL, GRP, SPLIT>(sh, wi, BN, a.grp_k);
+      const Item w = k_item<VL, GRP, SINKS>(sh, wi, BN, a.grp_k);
       if (w.total == 0) continue;
       if (!mbar_wait_warp(&bar_res, ai & 1, &abort_flag)) {
         if (lane == 0) raise_error(a.status, &abort_flag, kDevTimeoutTmaFull);
@@ -896,7 +902,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
     for (int j = 0; ok; ++j) {
       const int wi = snake_item(j, c, P);
       if (wi >= n_items) break;
-      const KItem w = k_item<VL, GRP, SPLIT>(sh, wi, BN, a.grp_k);
+      const Item w = k_item<VL, GRP, SINKS>(sh, wi, BN, a.grp_k);
       if (w.total == 0) continue;
       for (int it = 0; it < w.total; ++it, ++gt) {
         if (!mbar_wait_warp(&bar_ops_full, gt & 1, &abort_flag)) {
@@ -937,7 +943,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
     for (int j = 0; ok; ++j) {
       const int wi = snake_item(j, c, P);
       if (wi >= n_items) break;
-      const KItem w = k_item<VL, GRP, SPLIT>(sh, wi, BN, a.grp_k);
+      const Item w = k_item<VL, GRP, SINKS>(sh, wi, BN, a.grp_k);
       const int key = w.k0 + r;
       const bool key_ok = key < w.l.Tk;
       const int qhi = query_hi(w.l, key), qlo = query_lo(w.l, key);  // queries that see this key
@@ -945,10 +951,13 @@ __global__ void __launch_bounds__(kBBThreads, 1)
       __nv_bfloat16* dst = (wg == 0 ? a.dk2 : a.dv2) + k_row(w.l, w.r, skey, w.hk);
       if (w.total == 0) {
         // No query sees these keys (causal with Tk > Tq): the gradients are zero.
-        if (SPLIT && w.part >= 0)
-          zero_row_f32<HD>(sink_part_row(sh, HD, w.k0 / kBM, w.b * sh.Hk + w.hk, w.part, wg, r));
-        else if (key_ok)
-          zero_row_global<HD>(dst);
+        if constexpr (SPLIT) {
+          if (w.part >= 0) {
+            zero_row_f32<HD>(sink_part_row(sh, HD, w.k0 / kBM, w.b * sh.Hk + w.hk, w.part, wg, r));
+            continue;
+          }
+        }
+        if (key_ok) zero_row_global<HD>(dst);
         continue;
       }
       // head_dim 128: this item's ddV rows into TMEM, each warpgroup half of the head_dim columns, once
@@ -999,11 +1008,15 @@ __global__ void __launch_bounds__(kBBThreads, 1)
         break;
       }
       tc_fence_after();
-      if (SPLIT && w.part >= 0)
-        tmem_row_to_f32<HD>(tmem, warp, wg == 0 ? G::C_DK : G::C_DV,
-                            sink_part_row(sh, HD, w.k0 / kBM, w.b * sh.Hk + w.hk, w.part, wg, r), key_ok,
-                            wg == 0 ? sc : 1.f);
-      else
+      bool whole = true;
+      if constexpr (SPLIT) {
+        whole = w.part < 0;
+        if (!whole)
+          tmem_row_to_f32<HD>(tmem, warp, wg == 0 ? G::C_DK : G::C_DV,
+                              sink_part_row(sh, HD, w.k0 / kBM, w.b * sh.Hk + w.hk, w.part, wg, r), key_ok,
+                              wg == 0 ? sc : 1.f);
+      }
+      if (whole)
         tmem_row_to_global<HD>(tmem, warp, wg == 0 ? G::C_DK : G::C_DV, dst, key_ok, wg == 0 ? sc : 1.f);
       warp_arrive(&bar_acc_empty);  // the accumulators may be overwritten by the next item
       ++ai;
@@ -1016,7 +1029,7 @@ __global__ void __launch_bounds__(kBBThreads, 1)
 }
 
 template <int HD, bool VL>
-int launch_bwdbwd_hd(const AttnShape& s, const BwdBwdPtrs& p, int passes, int* status, cudaStream_t stream) {
+int launch_bwdbwd_hd(const SinkShape& s, const BwdBwdPtrs& p, int passes, int* status, cudaStream_t stream) {
   using GQ = QPass<HD>;
   using GK = KPass<HD>;
   CUtensorMap mq[8], mk[7];
@@ -1040,81 +1053,88 @@ int launch_bwdbwd_hd(const AttnShape& s, const BwdBwdPtrs& p, int passes, int* s
        make_seq_map(&mk[5], p.dO ? p.dO : p.q, HD, s.total_q, s.H, map_batch(s), s.sq, GK::BN) &&
        make_seq_map(&mk[6], p.ddq, HD, s.total_q, s.H, map_batch(s), s.sq, GK::BN);
   if (!ok) return kInvalidArgument;
-  // With `o`, the query pass computes D into delta_out and the key pass reads it there.
-  BBArgs args{s,
-              p.lse,
-              p.o ? p.delta_out : p.delta,
-              p.o ? p.delta_out : nullptr,
-              p.dd,
-              p.bv,
-              static_cast<__nv_bfloat16*>(p.dq2),
-              static_cast<__nv_bfloat16*>(p.ddo),
-              static_cast<__nv_bfloat16*>(p.dk2),
-              static_cast<__nv_bfloat16*>(p.dv2),
-              status};
   // Shared streamed tiles per head: K, V, ddK, ddV of a key head for the query pass;
   // Q, ddQ and dO of its query heads for the key pass.
   const int G = s.H / s.Hk;
-  args.grp_q = locality_group(s.H * s.B, G, 4ll * s.Tk * HD * 2);
-  args.grp_k = locality_group(s.Hk * s.B, 1, 3ll * G * s.Tq * HD * 2);
+  const int group_q = locality_group(s.H * s.B, G, 4ll * s.Tk * HD * 2);
+  const int group_k = locality_group(s.Hk * s.B, 1, 3ll * G * s.Tq * HD * 2);
+  // With `o`, the query pass computes D into delta_out and the key pass reads it there.
+  auto make_args = [&](auto snk) {
+    return BBArgs<decltype(snk)::value>{s,
+                                        p.lse,
+                                        p.o ? p.delta_out : p.delta,
+                                        p.o ? p.delta_out : nullptr,
+                                        p.dd,
+                                        p.bv,
+                                        static_cast<__nv_bfloat16*>(p.dq2),
+                                        static_cast<__nv_bfloat16*>(p.ddo),
+                                        static_cast<__nv_bfloat16*>(p.dk2),
+                                        static_cast<__nv_bfloat16*>(p.dv2),
+                                        status,
+                                        group_q,
+                                        group_k};
+  };
   // The grouped kernels only where the groups split the pairs (packed ragged batches
   // keep the plain order). The persistent key pass groups only equal-weight items (no
   // causal mask): its static snake balances work only over a heaviest-first sequence,
   // which a grouped causal order is not (measured: key pass 2.24 -> 3.00 ms at causal
   // B1 H32 S8192 D128), while the query pass is balanced by the block scheduler.
-  // With sinks the query tiles of a head share few of their keys: plain order.
-  const bool grp_q = !VL && s.sinks == 0 && args.grp_q < s.H * s.B;
-  const bool grp_k = !VL && !s.causal && args.grp_k < s.Hk * s.B;
-  const int nq = (s.Tq + kBM - 1) / kBM;
+  const bool grp_q = !VL && group_q < s.H * s.B, grp_k = !VL && !s.causal && group_k < s.Hk * s.B;
+  const int nq = (s.Tq + kBM - 1) / kBM, nk = (s.Tk + kBM - 1) / kBM;
   const dim3 gq(s.H, s.B, nq), gq_grouped(s.H * s.B * nq);
-  auto launch_q = [&](auto* kernel, dim3 grid) {
+  // The key pass is persistent: one CTA per SM (at most one per work item).
+  const int items = s.Hk * s.B * (s.splits > 1 ? split_slots(s, nk) : nk);
+  const dim3 gk(static_cast<unsigned>(items < sm_count() ? items : sm_count()));
+  auto launch_q = [&](auto* kernel, dim3 grid, const auto& args) {
     if (ensure_smem_limit(reinterpret_cast<const void*>(kernel), GQ::SMEM) != kOk) return kLaunchFailed;
     kernel<<<grid, kBBThreads, GQ::SMEM, stream>>>(mq[0], mq[1], mq[2], mq[3], mq[4], mq[5], mq[6], mq[7], args);
     return static_cast<HostStatus>(after_launch());
   };
-  auto launch_k = [&](auto* kernel, dim3 grid) {
+  auto launch_k = [&](auto* kernel, const auto& args) {
     if (ensure_smem_limit(reinterpret_cast<const void*>(kernel), GK::SMEM) != kOk) return kLaunchFailed;
-    kernel<<<grid, kBBThreads, GK::SMEM, stream>>>(mk[0], mk[1], mk[2], mk[3], mk[4], mk[5], mk[6], args);
+    kernel<<<gk, kBBThreads, GK::SMEM, stream>>>(mk[0], mk[1], mk[2], mk[3], mk[4], mk[5], mk[6], args);
     return static_cast<HostStatus>(after_launch());
   };
+  const bool tj = (passes & kPassFwdTangent) != 0;
+  if (s.sinks > 0) {  // plain order: the query tiles of a head share few of their keys
+    const auto args = make_args(std::true_type{});
+    HostStatus rc = kOk;
+    if (passes & (kPassFwdTangent | kPassQuery))
+      rc = tj ? launch_q(&bwdbwd_q_kernel<HD, VL, true, false, true>, gq, args)
+              : launch_q(&bwdbwd_q_kernel<HD, VL, false, false, true>, gq, args);
+    if (rc != kOk || !(passes & kPassKey)) return rc;
+    if (s.splits == 1) return launch_k(&bwdbwd_k_kernel<HD, VL, false, kSinksWhole>, args);
+    rc = launch_k(&bwdbwd_k_kernel<HD, VL, false, kSinksSplit>, args);
+    return rc != kOk ? rc : launch_sink_join(s, HD, p.dk2, p.dv2, nullptr, nullptr, stream);
+  }
+  const auto args = make_args(std::false_type{});
   if (passes & (kPassFwdTangent | kPassQuery)) {
-    const bool tj = (passes & kPassFwdTangent) != 0;
     HostStatus rc = kOk;
     bool done = false;
     if constexpr (!VL) {
       if (grp_q) {
-        rc = tj ? launch_q(&bwdbwd_q_kernel<HD, false, true, true, false>, gq_grouped)
-                : launch_q(&bwdbwd_q_kernel<HD, false, false, true, false>, gq_grouped);
+        rc = tj ? launch_q(&bwdbwd_q_kernel<HD, false, true, true, false>, gq_grouped, args)
+                : launch_q(&bwdbwd_q_kernel<HD, false, false, true, false>, gq_grouped, args);
         done = true;
       }
     }
-    if (!done && s.sinks > 0)
-      rc = tj ? launch_q(&bwdbwd_q_kernel<HD, VL, true, false, true>, gq)
-              : launch_q(&bwdbwd_q_kernel<HD, VL, false, false, true>, gq);
-    else if (!done)
-      rc = tj ? launch_q(&bwdbwd_q_kernel<HD, VL, true, false, false>, gq)
-              : launch_q(&bwdbwd_q_kernel<HD, VL, false, false, false>, gq);
+    if (!done)
+      rc = tj ? launch_q(&bwdbwd_q_kernel<HD, VL, true, false, false>, gq, args)
+              : launch_q(&bwdbwd_q_kernel<HD, VL, false, false, false>, gq, args);
     if (rc != kOk) return rc;
   }
   if (passes & kPassKey) {
-    // Persistent: one CTA per SM (at most one per work item).
-    const int nk = (s.Tk + kBM - 1) / kBM, items = s.Hk * s.B * (s.splits > 1 ? split_slots(s, nk) : nk);
-    const dim3 gk(static_cast<unsigned>(items < sm_count() ? items : sm_count()));
-    if (s.splits > 1) {
-      const HostStatus rc = launch_k(&bwdbwd_k_kernel<HD, VL, false, true>, gk);
-      return rc != kOk ? rc : launch_sink_join(s, HD, p.dk2, p.dv2, nullptr, nullptr, stream);
-    }
     if constexpr (!VL) {
-      if (grp_k) return launch_k(&bwdbwd_k_kernel<HD, false, true, false>, gk);
+      if (grp_k) return launch_k(&bwdbwd_k_kernel<HD, false, true, kNoSinks>, args);
     }
-    return launch_k(&bwdbwd_k_kernel<HD, VL, false, false>, gk);
+    return launch_k(&bwdbwd_k_kernel<HD, VL, false, kNoSinks>, args);
   }
   return kOk;
 }
 
 }  // namespace
 
-int launch_bwdbwd(const AttnShape& s, int hd, const BwdBwdPtrs& p, int passes, int* status, cudaStream_t stream) {
+int launch_bwdbwd(const SinkShape& s, int hd, const BwdBwdPtrs& p, int passes, int* status, cudaStream_t stream) {
   if (hd == 64) return s.cu_q ? launch_bwdbwd_hd<64, true>(s, p, passes, status, stream) : launch_bwdbwd_hd<64, false>(s, p, passes, status, stream);
   if (hd == 128) return s.cu_q ? launch_bwdbwd_hd<128, true>(s, p, passes, status, stream) : launch_bwdbwd_hd<128, false>(s, p, passes, status, stream);
   return kUnsupported;

@@ -107,7 +107,7 @@ bool strides_ok(const fh_strides& s) {
   return s.batch >= 0 && s.seq > 0 && s.head >= 0 && s.batch % 8 == 0 && s.seq % 8 == 0 && s.head % 8 == 0;
 }
 
-int validate(const fh_attn_dims* d, AttnShape* out, float scale, int causal, bool allow_varlen = true) {
+int validate(const fh_attn_dims* d, SinkShape* out, float scale, int causal, bool allow_varlen = true) {
   g_last_error[0] = 0;
   if (!d) return fail(kInvalidArgument, "dims is NULL");
   const bool varlen = d->cu_seqlens_q != nullptr || d->cu_seqlens_k != nullptr;
@@ -257,7 +257,7 @@ const char* fh_status_string(int status) {
 }
 
 long long fh_attn_sink_scratch_floats(const fh_attn_dims* dims, int causal) {
-  AttnShape s;
+  SinkShape s;
   if (validate(dims, &s, 1.f, causal) != kOk) return -1;
   return sink_part_floats(s, dims->head_dim, sink_splits(s));
 }
@@ -265,7 +265,7 @@ long long fh_attn_sink_scratch_floats(const fh_attn_dims* dims, int causal) {
 int fh_attn_fwd(void* stream, const fh_attn_dims* dims, const void* q, const void* k, const void* v, void* o,
                 float* lse, float scale, int causal) {
   if (injected("fh_attn_fwd")) return FH_ERR_INJECTED;
-  AttnShape s;
+  SinkShape s;
   int rc = validate(dims, &s, scale, causal);
   if (rc != kOk) return rc;
   if (!all_aligned(q, k, v, o) || !lse) return fail(FH_ERR_INVALID_ARGUMENT, kAlignMsg);
@@ -278,7 +278,7 @@ int fh_attn_fwd(void* stream, const fh_attn_dims* dims, const void* q, const voi
 
 int fh_attn_rowdot(void* stream, const fh_attn_dims* dims, const void* o, const void* dO, float* delta) {
   if (injected("fh_attn_rowdot")) return FH_ERR_INJECTED;
-  AttnShape s;
+  SinkShape s;
   int rc = validate(dims, &s, 1.f, 0);
   if (rc != kOk) return rc;
   if (!all_aligned(o, dO) || !delta) return fail(FH_ERR_INVALID_ARGUMENT, kAlignMsg);
@@ -291,7 +291,7 @@ int fh_attn_bwd(void* stream, const fh_attn_dims* dims, const void* q, const voi
                 const void* dO, const float* lse, void* dq, void* dk, void* dv, float* delta, float scale,
                 int causal) {
   if (injected("fh_attn_bwd")) return FH_ERR_INJECTED;
-  AttnShape s;
+  SinkShape s;
   int rc = validate(dims, &s, scale, causal);
   if (rc != kOk) return rc;
   if (!all_aligned(q, k, v, o, dO, dq, dk, dv) || !lse || !delta) return fail(FH_ERR_INVALID_ARGUMENT, kAlignMsg);
@@ -309,7 +309,7 @@ static int bwdbwd_entry(const char* entry, void* stream, const fh_attn_dims* dim
                         const void* ddv, const float* lse, const float* delta, float* delta_out, void* dq2, void* ddo,
                         void* dk2, void* dv2, float* dd, float* bvec, float scale, int causal, int passes) {
   if (injected(entry)) return FH_ERR_INJECTED;
-  AttnShape s;
+  SinkShape s;
   int rc = validate(dims, &s, scale, causal);
   if (rc != kOk) return rc;
   if (passes == kPassFwdTangent) {
@@ -369,7 +369,7 @@ int fh_attn_jvp_bwd(void* stream, const fh_attn_dims* dims, const void* q, const
                     const void* tdO, void* tdq, void* tdk, void* tdv, void* to, float* delta, float* dd, float* bvec,
                     float scale, int causal) {
   if (injected("fh_attn_jvp_bwd")) return FH_ERR_INJECTED;
-  AttnShape s;
+  SinkShape s;
   int rc = validate(dims, &s, scale, causal);
   if (rc != kOk) return rc;
   if (!all_aligned(q, k, v, o, dO, tq, tk, tv, tdq, tdk, tdv, to) || !lse || !delta || !dd || !bvec)
@@ -395,7 +395,7 @@ int fh_attn_jvp_bwd(void* stream, const fh_attn_dims* dims, const void* q, const
 int fh_attn_fwd_f32(void* stream, const fh_attn_dims* dims, const float* q, const float* k, const float* v,
                     float* o, float* lse, float scale, int causal) {
   if (injected("fh_attn_fwd_f32")) return FH_ERR_INJECTED;
-  AttnShape s;
+  SinkShape s;
   int rc = validate(dims, &s, scale, causal, false);
   if (rc != kOk) return rc;
   if (!all_aligned(q, k, v, o) || !lse) return fail(FH_ERR_INVALID_ARGUMENT, kAlignMsg);
@@ -408,7 +408,7 @@ int fh_attn_bwd_f32(void* stream, const fh_attn_dims* dims, const float* q, cons
                     const float* o, const float* dO, const float* lse, float* dq, float* dk, float* dv, float* delta,
                     float scale, int causal) {
   if (injected("fh_attn_bwd_f32")) return FH_ERR_INJECTED;
-  AttnShape s;
+  SinkShape s;
   int rc = validate(dims, &s, scale, causal, false);
   if (rc != kOk) return rc;
   if (!all_aligned(q, k, v, o, dO, dq, dk, dv) || !lse || !delta) return fail(FH_ERR_INVALID_ARGUMENT, kAlignMsg);
@@ -422,7 +422,7 @@ int fh_attn_bwdbwd_f32(void* stream, const fh_attn_dims* dims, const float* q, c
                        const float* lse, float* dq2, float* ddo, float* dk2, float* dv2, float* delta, float* dd,
                        float* bvec, float scale, int causal, int passes) {
   if (injected("fh_attn_bwdbwd_f32")) return FH_ERR_INJECTED;
-  AttnShape s;
+  SinkShape s;
   int rc = validate(dims, &s, scale, causal, false);
   if (rc != kOk) return rc;
   if (passes < 1 || passes > 3) return fail(FH_ERR_INVALID_ARGUMENT, "pass must be 1, 2 or 3");
@@ -443,7 +443,7 @@ int fh_attn_jvp_bwd_f32(void* stream, const fh_attn_dims* dims, const float* q, 
                         const float* tv, const float* tdO, float* tdq, float* tdk, float* tdv, float* to,
                         float* delta, float* dd, float* bvec, float scale, int causal) {
   if (injected("fh_attn_jvp_bwd_f32")) return FH_ERR_INJECTED;
-  AttnShape s;
+  SinkShape s;
   int rc = validate(dims, &s, scale, causal, false);
   if (rc != kOk) return rc;
   if (!all_aligned(q, k, v, o, dO, tq, tk, tv, tdq, tdk, tdv, to) || !lse || !delta || !dd || !bvec)
@@ -790,7 +790,7 @@ extern "C" int fh_attn_bwdbwd_noalloc(void* stream, const fh_attn_dims* dims, co
                                       const void* ddk, const void* ddv, const float* lse, void* dq2, void* ddo,
                                       void* dk2, void* dv2, float scale, int causal, int* device_status) {
   if (injected("fh_attn_bwdbwd_noalloc")) return FH_ERR_INJECTED;
-  AttnShape s;
+  SinkShape s;
   int rc = validate(dims, &s, scale, causal);
   if (rc != kOk) return rc;
   const long long rows = static_cast<long long>(s.cu_q ? 1 : s.B) * s.H * s.total_q;

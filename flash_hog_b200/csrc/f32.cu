@@ -61,6 +61,9 @@ __device__ __forceinline__ float max16(float x) {
 }
 
 __device__ __forceinline__ bool visible(const AttnShape& s, int i, int j) {
+  return i < s.Tq && j < s.Tk && j >= key_lo(s, i) && j <= key_hi(s, i);
+}
+__device__ __forceinline__ bool visible(const SinkShape& s, int i, int j) {
   return i < s.Tq && j < s.Tk && j <= key_hi(s, i) && (j >= key_lo(s, i) || j < s.sinks);
 }
 
@@ -281,9 +284,9 @@ constexpr int kFwdCtas = 2;
 template <int HD>
 constexpr int kDkdvCtas = HD == 64 ? 2 : 1;
 
-template <int HD>
+template <int HD, bool SNK>
 __global__ void __launch_bounds__(kThreads, kFwdCtas<HD>)
-    fwd_kernel(AttnShape s, const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
+    fwd_kernel(ShapeOf<SNK> s, const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
                float* __restrict__ o, float* __restrict__ lse) {
   using G = Geo<HD>;
   extern __shared__ float4 smem_f4[];
@@ -299,16 +302,20 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas<HD>)
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = -INFINITY, l[i] = 0.f;
   zero(acc);
-  const SinkTiles tiles = sink_key_tiles(s, r0, kRes, G::BN);
-  const int nt = tiles.n;
+  int first;
+  SinkTiles sink{0, 0, 0};
+  if constexpr (SNK) sink = sink_key_tiles(s, r0, kRes, G::BN);
+  // Key tiles first, first + 1, ... or, with sinks, sink.tile(0), ...
+  const int nt = SNK ? sink.n : key_tiles(s, r0, kRes, G::BN, &first);
+  auto tile_of = [&](int it) { return SNK ? sink.tile(it) : first + it; };
   auto fetch = [&](int t) {
     float* buf = sKV + (t & 1) * 2 * G::STR;
-    load_rows_async<HD, G::BN>(buf, k, s.sk, b, hk, tiles.tile(t) * G::BN, s.Tk);
-    load_rows_async<HD, G::BN>(buf + G::STR, v, s.sk, b, hk, tiles.tile(t) * G::BN, s.Tk);
+    load_rows_async<HD, G::BN>(buf, k, s.sk, b, hk, tile_of(t) * G::BN, s.Tk);
+    load_rows_async<HD, G::BN>(buf + G::STR, v, s.sk, b, hk, tile_of(t) * G::BN, s.Tk);
   };
   if (nt > 0) fetch(0);
   for (int it = 0; it < nt; ++it) {
-    const int c0 = tiles.tile(it) * G::BN;
+    const int c0 = tile_of(it) * G::BN;
     // Buffer (it + 1) & 1 was last read in iteration it - 1, which ended with a barrier.
     if (it + 1 < nt) {
       fetch(it + 1);
@@ -385,9 +392,9 @@ __global__ void __launch_bounds__(kThreads)
 // cuDNN): P = exp(scale S - L), dS = scale P o (dO V^T - D);
 //   query side: dQ = dS K;   key side: dV = P^T dO, dK = dS^T Q.
 // ------------------------------------------------------------------------------------
-template <int HD>
+template <int HD, bool SNK>
 __global__ void __launch_bounds__(kThreads, kFwdCtas<HD>)
-    dq_kernel(AttnShape s, const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
+    dq_kernel(ShapeOf<SNK> s, const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
               const float* __restrict__ dO, const float* __restrict__ lse, const float* __restrict__ delta,
               float* __restrict__ dq, const float* dq_acc) {
   using G = Geo<HD>;
@@ -410,10 +417,14 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas<HD>)
   }
   float acc[4][G::NO];
   zero(acc);
-  const SinkTiles tiles = sink_key_tiles(s, r0, kRes, G::BN);
-  const int nt = tiles.n;
+  int first;
+  SinkTiles sink{0, 0, 0};
+  if constexpr (SNK) sink = sink_key_tiles(s, r0, kRes, G::BN);
+  // Key tiles first, first + 1, ... or, with sinks, sink.tile(0), ...
+  const int nt = SNK ? sink.n : key_tiles(s, r0, kRes, G::BN, &first);
+  auto tile_of = [&](int it) { return SNK ? sink.tile(it) : first + it; };
   for (int it = 0; it < nt; ++it) {
-    const int c0 = tiles.tile(it) * G::BN;
+    const int c0 = tile_of(it) * G::BN;
     __syncthreads();
     load_rows<HD, G::BN>(sK, k, s.sk, b, hk, c0, s.Tk);
     load_rows<HD, G::BN>(sV, v, s.sk, b, hk, c0, s.Tk);
@@ -438,9 +449,9 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas<HD>)
   store_rows<HD>(dq, dq_acc, s.sq, b, h, r0, s.Tq, acc, one, rg, cg);
 }
 
-template <int HD>
+template <int HD, bool SNK>
 __global__ void __launch_bounds__(kThreads, kDkdvCtas<HD>)
-    dkdv_kernel(AttnShape s, const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
+    dkdv_kernel(ShapeOf<SNK> s, const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
                 const float* __restrict__ dO, const float* __restrict__ lse, const float* __restrict__ delta,
                 float* __restrict__ dk, float* __restrict__ dv, const float* dk_acc, const float* dv_acc) {
   using G = Geo<HD>;
@@ -508,9 +519,9 @@ __global__ void __launch_bounds__(kThreads, kDkdvCtas<HD>)
 //   B = rowsum(P o X) - dD rowsum(P o dP) - D dD + rowsum(P o dP o ddS),
 // so one sweep gathers all row statistics and a second sweep produces dQ' and ddO.
 // ------------------------------------------------------------------------------------
-template <int HD>
+template <int HD, bool SNK>
 __global__ void __launch_bounds__(kThreads, 1)
-    bbq_kernel(AttnShape s, const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
+    bbq_kernel(ShapeOf<SNK> s, const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
                const float* __restrict__ dO, const float* __restrict__ ddq, const float* __restrict__ ddk,
                const float* __restrict__ ddv, const float* __restrict__ lse, const float* __restrict__ delta,
                float* __restrict__ dq2, float* __restrict__ ddo, float* __restrict__ dd_out,
@@ -537,15 +548,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     L[i] = row < s.Tq ? lse[stat_index(s, b, h, row)] : 0.f;
     D[i] = row < s.Tq ? delta[stat_index(s, b, h, row)] : 0.f;
   }
-  const SinkTiles tiles = sink_key_tiles(s, r0, kRes, G::BN);
-  const int nt = tiles.n;
+  int first;
+  SinkTiles sink{0, 0, 0};
+  if constexpr (SNK) sink = sink_key_tiles(s, r0, kRes, G::BN);
+  // Key tiles first, first + 1, ... or, with sinks, sink.tile(0), ...
+  const int nt = SNK ? sink.n : key_tiles(s, r0, kRes, G::BN, &first);
+  auto tile_of = [&](int it) { return SNK ? sink.tile(it) : first + it; };
 
   // Items u = 0 .. 2 nt - 1: sweep 1 (row statistics) over the key tiles, then sweep 2
   // (dQ', ddO) over the same tiles. With two buffers, item u + 1's tile is fetched
   // (cp.async) while item u's is used, across the sweep boundary too.
   const int total = 2 * nt;
   auto fetch = [&](int u) {
-    const int c0 = tiles.tile(u % nt) * G::BN;
+    const int c0 = tile_of(u % nt) * G::BN;
     float* buf = kbuf + (u % NBUF) * BUF;
     load_rows_async<HD, G::BN>(buf, k, s.sk, b, hk, c0, s.Tk);
     load_rows_async<HD, G::BN>(buf + G::STR, v, s.sk, b, hk, c0, s.Tk);
@@ -574,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (NBUF == 2 && total > 0) fetch(0);
   for (int u = 0; u < total; ++u) {
-    const int c0 = tiles.tile(u % nt) * G::BN;
+    const int c0 = tile_of(u % nt) * G::BN;
     if (NBUF == 2) {
       // Buffer (u + 1) % 2 was last read in item u - 1, which ended with a barrier.
       if (u + 1 < total) {
@@ -662,9 +677,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   store_rows<HD>(ddo, nullptr, s.sq, b, h, r0, s.Tq, ao, one, rg, cg);
 }
 
-template <int HD>
+template <int HD, bool SNK>
 __global__ void __launch_bounds__(kThreads, 1)
-    bbk_kernel(AttnShape s, const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
+    bbk_kernel(ShapeOf<SNK> s, const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
                const float* __restrict__ dO, const float* __restrict__ ddq, const float* __restrict__ ddk,
                const float* __restrict__ ddv, const float* __restrict__ lse, const float* __restrict__ delta,
                const float* __restrict__ dd, const float* __restrict__ bvec, float* __restrict__ dk2,
@@ -806,11 +821,11 @@ static_assert(smem_bbq<128>() <= 232448 && smem_bbk<128>() <= 232448, "shared me
 inline dim3 query_grid(const AttnShape& s) { return dim3((s.Tq + kRes - 1) / kRes, s.H, s.B); }
 inline dim3 key_grid(const AttnShape& s) { return dim3((s.Tk + kRes - 1) / kRes, s.Hk, s.B); }
 
-template <int HD>
-int fwd(const AttnShape& s, const F32FwdPtrs& p, cudaStream_t st) {
+template <int HD, bool SNK>
+int fwd(const SinkShape& s, const F32FwdPtrs& p, cudaStream_t st) {
   constexpr int sm = smem_fwd<HD>();
-  if (ensure_smem_limit(reinterpret_cast<const void*>(&fwd_kernel<HD>), sm) != kOk) return kLaunchFailed;
-  fwd_kernel<HD><<<query_grid(s), kThreads, sm, st>>>(s, p.q, p.k, p.v, p.o, p.lse);
+  if (ensure_smem_limit(reinterpret_cast<const void*>(&fwd_kernel<HD, SNK>), sm) != kOk) return kLaunchFailed;
+  fwd_kernel<HD, SNK><<<query_grid(s), kThreads, sm, st>>>(s, p.q, p.k, p.v, p.o, p.lse);
   return after_launch();
 }
 
@@ -823,35 +838,35 @@ int rowdot(const AttnShape& s, const float* o, const float* dO, float* delta, cu
   return after_launch();
 }
 
-template <int HD>
-int bwd(const AttnShape& s, const F32BwdPtrs& p, cudaStream_t st) {
+template <int HD, bool SNK>
+int bwd(const SinkShape& s, const F32BwdPtrs& p, cudaStream_t st) {
   int rc = rowdot<HD>(s, p.o, p.dO, p.delta, st);
   if (rc != kOk) return rc;
   constexpr int sq = smem_dq<HD>(), sk = smem_dkdv<HD>();
-  if (ensure_smem_limit(reinterpret_cast<const void*>(&dq_kernel<HD>), sq) != kOk) return kLaunchFailed;
-  if (ensure_smem_limit(reinterpret_cast<const void*>(&dkdv_kernel<HD>), sk) != kOk) return kLaunchFailed;
-  dq_kernel<HD><<<query_grid(s), kThreads, sq, st>>>(s, p.q, p.k, p.v, p.dO, p.lse, p.delta, p.dq, p.dq_acc);
+  if (ensure_smem_limit(reinterpret_cast<const void*>(&dq_kernel<HD, SNK>), sq) != kOk) return kLaunchFailed;
+  if (ensure_smem_limit(reinterpret_cast<const void*>(&dkdv_kernel<HD, SNK>), sk) != kOk) return kLaunchFailed;
+  dq_kernel<HD, SNK><<<query_grid(s), kThreads, sq, st>>>(s, p.q, p.k, p.v, p.dO, p.lse, p.delta, p.dq, p.dq_acc);
   if ((rc = after_launch()) != kOk) return rc;
-  dkdv_kernel<HD><<<key_grid(s), kThreads, sk, st>>>(s, p.q, p.k, p.v, p.dO, p.lse, p.delta, p.dk, p.dv, p.dk_acc,
+  dkdv_kernel<HD, SNK><<<key_grid(s), kThreads, sk, st>>>(s, p.q, p.k, p.v, p.dO, p.lse, p.delta, p.dk, p.dv, p.dk_acc,
                                                       p.dv_acc);
   return after_launch();
 }
 
-template <int HD>
-int bwdbwd(const AttnShape& s, const F32BwdBwdPtrs& p, int passes, cudaStream_t st) {
+template <int HD, bool SNK>
+int bwdbwd(const SinkShape& s, const F32BwdBwdPtrs& p, int passes, cudaStream_t st) {
   int rc = kOk;
   if (passes & kPassQuery) {
     if ((rc = rowdot<HD>(s, p.o, p.dO, p.delta, st)) != kOk) return rc;
     constexpr int sm = smem_bbq<HD>();
-    if (ensure_smem_limit(reinterpret_cast<const void*>(&bbq_kernel<HD>), sm) != kOk) return kLaunchFailed;
-    bbq_kernel<HD><<<query_grid(s), kThreads, sm, st>>>(s, p.q, p.k, p.v, p.dO, p.ddq, p.ddk, p.ddv, p.lse, p.delta,
+    if (ensure_smem_limit(reinterpret_cast<const void*>(&bbq_kernel<HD, SNK>), sm) != kOk) return kLaunchFailed;
+    bbq_kernel<HD, SNK><<<query_grid(s), kThreads, sm, st>>>(s, p.q, p.k, p.v, p.dO, p.ddq, p.ddk, p.ddv, p.lse, p.delta,
                                                          p.dq2, p.ddo, p.dd, p.bv);
     if ((rc = after_launch()) != kOk) return rc;
   }
   if (passes & kPassKey) {
     constexpr int sm = smem_bbk<HD>();
-    if (ensure_smem_limit(reinterpret_cast<const void*>(&bbk_kernel<HD>), sm) != kOk) return kLaunchFailed;
-    bbk_kernel<HD><<<key_grid(s), kThreads, sm, st>>>(s, p.q, p.k, p.v, p.dO, p.ddq, p.ddk, p.ddv, p.lse, p.delta,
+    if (ensure_smem_limit(reinterpret_cast<const void*>(&bbk_kernel<HD, SNK>), sm) != kOk) return kLaunchFailed;
+    bbk_kernel<HD, SNK><<<key_grid(s), kThreads, sm, st>>>(s, p.q, p.k, p.v, p.dO, p.ddq, p.ddk, p.ddv, p.lse, p.delta,
                                                        p.dd, p.bv, p.dk2, p.dv2);
     rc = after_launch();
   }
@@ -860,16 +875,19 @@ int bwdbwd(const AttnShape& s, const F32BwdBwdPtrs& p, int passes, cudaStream_t 
 
 }  // namespace f32
 
-int launch_fwd_f32(const AttnShape& s, int hd, const F32FwdPtrs& p, cudaStream_t stream) {
-  return hd == 64 ? f32::fwd<64>(s, p, stream) : f32::fwd<128>(s, p, stream);
+int launch_fwd_f32(const SinkShape& s, int hd, const F32FwdPtrs& p, cudaStream_t stream) {
+  if (s.sinks > 0) return hd == 64 ? f32::fwd<64, true>(s, p, stream) : f32::fwd<128, true>(s, p, stream);
+  return hd == 64 ? f32::fwd<64, false>(s, p, stream) : f32::fwd<128, false>(s, p, stream);
 }
 
-int launch_bwd_f32(const AttnShape& s, int hd, const F32BwdPtrs& p, cudaStream_t stream) {
-  return hd == 64 ? f32::bwd<64>(s, p, stream) : f32::bwd<128>(s, p, stream);
+int launch_bwd_f32(const SinkShape& s, int hd, const F32BwdPtrs& p, cudaStream_t stream) {
+  if (s.sinks > 0) return hd == 64 ? f32::bwd<64, true>(s, p, stream) : f32::bwd<128, true>(s, p, stream);
+  return hd == 64 ? f32::bwd<64, false>(s, p, stream) : f32::bwd<128, false>(s, p, stream);
 }
 
-int launch_bwdbwd_f32(const AttnShape& s, int hd, const F32BwdBwdPtrs& p, int passes, cudaStream_t stream) {
-  return hd == 64 ? f32::bwdbwd<64>(s, p, passes, stream) : f32::bwdbwd<128>(s, p, passes, stream);
+int launch_bwdbwd_f32(const SinkShape& s, int hd, const F32BwdBwdPtrs& p, int passes, cudaStream_t stream) {
+  if (s.sinks > 0) return hd == 64 ? f32::bwdbwd<64, true>(s, p, passes, stream) : f32::bwdbwd<128, true>(s, p, passes, stream);
+  return hd == 64 ? f32::bwdbwd<64, false>(s, p, passes, stream) : f32::bwdbwd<128, false>(s, p, passes, stream);
 }
 
 }  // namespace fh

@@ -39,8 +39,9 @@
 namespace fh {
 namespace {
 
+template <bool SNK>
 struct FwdArgs {
-  AttnShape sh;
+  ShapeOf<SNK> sh;
   __nv_bfloat16* o;
   float* lse;
   int* status;
@@ -117,7 +118,7 @@ __device__ __forceinline__ void fwd_warp_arrive(uint64_t* bar) {
 template <int HD, bool VL, bool GRP, bool SNK>
 __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
     fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-               const __grid_constant__ CUtensorMap tm_v, const FwdArgs a) {
+               const __grid_constant__ CUtensorMap tm_v, const FwdArgs<SNK> a) {
   using G = FPass<HD>;
   constexpr int BN = G::BN, ST = G::ST, T = G::T;
   constexpr bool SEP_P = G::SEP_P;
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
     h = hb % a.sh.H, b = hb / a.sh.H, qt = nq - 1 - qi;
   }
   SeqRange sr;
-  const AttnShape sh = seq_shape<VL>(a.sh, b, &sr);  // this sequence's lengths and mask; sr: where its rows start
+  const ShapeOf<SNK> sh = seq_shape<VL>(a.sh, b, &sr);  // this sequence's lengths and mask; sr: where its rows start
   const int q0 = qt * G::ROWS;
   // Key tiles of each query tile: nt[t] tiles from key tile jt[t] (0 when the
   // tile lies past the last query row or sees no key). The ring streams the
@@ -342,10 +343,10 @@ __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
 #pragma unroll
       for (int i = 0; i < BN; ++i) asm volatile("" : "+r"(v[i])::"memory");
       if constexpr (G::SEP_P) fwd_warp_arrive(&bar_s_empty[t]);  // S(j+1) may be computed now
-      if (k0 + BN - 1 > khi || (k0 < klo && (!SNK || k0 + BN > sh.sinks))) {
+      if (k0 + BN - 1 > khi || (k0 < klo && (!SNK || k0 + BN > sinks_of(sh)))) {
 #pragma unroll
         for (int i = 0; i < BN; ++i)
-          if (k0 + i > khi || (k0 + i < klo && (!SNK || k0 + i >= sh.sinks))) v[i] = __float_as_uint(-INFINITY);
+          if (k0 + i > khi || (k0 + i < klo && (!SNK || k0 + i >= sinks_of(sh)))) v[i] = __float_as_uint(-INFINITY);
       }
       // Row maximum of the raw scores (the scale is positive), eight independent chains.
       float mx[8];
@@ -447,7 +448,7 @@ __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
 }
 
 template <int HD, bool VL>
-int launch_fwd_hd(const AttnShape& s, const FwdPtrs& p, int* status, cudaStream_t stream) {
+int launch_fwd_hd(const SinkShape& s, const FwdPtrs& p, int* status, cudaStream_t stream) {
   using G = FPass<HD>;
   CUtensorMap mq, mk, mv;
   if (!make_seq_map(&mq, p.q, HD, s.total_q, s.H, map_batch(s), s.sq, kBM) ||
@@ -455,26 +456,27 @@ int launch_fwd_hd(const AttnShape& s, const FwdPtrs& p, int* status, cudaStream_
       !make_seq_map(&mv, p.v, HD, s.total_k, s.Hk, map_batch(s), s.sk, G::BN))
     return kInvalidArgument;
   // K and V of a key head are the tiles the query tiles of its heads share.
-  FwdArgs args{s, static_cast<__nv_bfloat16*>(p.o), p.lse, status,
-               locality_group(s.H * s.B, s.H / s.Hk, 2ll * s.Tk * HD * 2)};
+  const int grp = locality_group(s.H * s.B, s.H / s.Hk, 2ll * s.Tk * HD * 2);
   const int nq = (s.Tq + G::ROWS - 1) / G::ROWS;
-  auto launch = [&](auto* kernel, dim3 grid) {
+  auto launch = [&](auto* kernel, dim3 grid, const auto& args) {
     if (ensure_smem_limit(reinterpret_cast<const void*>(kernel), G::SMEM) != kOk) return kLaunchFailed;
     kernel<<<grid, G::THREADS, G::SMEM, stream>>>(mq, mk, mv, args);
     return static_cast<HostStatus>(after_launch());
   };
   const dim3 grid(s.H, s.B, nq);
+  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.o);
   // Sinks: a query tile shares few of its keys with the head's other tiles, plain order.
-  if (s.sinks > 0) return launch(&fwd_kernel<HD, VL, false, true>, grid);
+  if (s.sinks > 0) return launch(&fwd_kernel<HD, VL, false, true>, grid, FwdArgs<true>{s, o, p.lse, status, grp});
+  const FwdArgs<false> args{s, o, p.lse, status, grp};
   if constexpr (!VL) {  // grouped only where the groups split the pairs
-    if (args.grp < s.H * s.B) return launch(&fwd_kernel<HD, false, true, false>, dim3(s.H * s.B * nq));
+    if (grp < s.H * s.B) return launch(&fwd_kernel<HD, false, true, false>, dim3(s.H * s.B * nq), args);
   }
-  return launch(&fwd_kernel<HD, VL, false, false>, grid);
+  return launch(&fwd_kernel<HD, VL, false, false>, grid, args);
 }
 
 }  // namespace
 
-int launch_fwd(const AttnShape& s, int hd, const FwdPtrs& p, int* status, cudaStream_t stream) {
+int launch_fwd(const SinkShape& s, int hd, const FwdPtrs& p, int* status, cudaStream_t stream) {
   if (hd == 64) return s.cu_q ? launch_fwd_hd<64, true>(s, p, status, stream) : launch_fwd_hd<64, false>(s, p, status, stream);
   if (hd == 128) return s.cu_q ? launch_fwd_hd<128, true>(s, p, status, stream) : launch_fwd_hd<128, false>(s, p, status, stream);
   return kUnsupported;

@@ -49,18 +49,18 @@ struct BwdBwdPtrs {
   float* delta_out = nullptr;
 };
 
-int launch_fwd(const AttnShape& s, int hd, const FwdPtrs& p, int* status, cudaStream_t stream);
+int launch_fwd(const SinkShape& s, int hd, const FwdPtrs& p, int* status, cudaStream_t stream);
 int launch_rowdot(const AttnShape& s, int hd, const void* o, const void* dO, float* delta, cudaStream_t stream);
-int launch_bwd(const AttnShape& s, int hd, const BwdPtrs& p, int* status, cudaStream_t stream);
+int launch_bwd(const SinkShape& s, int hd, const BwdPtrs& p, int* status, cudaStream_t stream);
 // passes: bitmask of kPassQuery (query-tiled: dQ', ddO, dD, B) and kPassKey (key-tiled: dK', dV'),
 // or kPassFwdTangent alone: the query-tiled pass for dO = 0 (ddO = the forward's tangent,
 // dD = the log-sum-exp's tangent; dO, O, delta, dq2 and bv are neither read nor written).
 enum BwdBwdPass : int { kPassQuery = 1, kPassKey = 2, kPassFwdTangent = 4 };
-int launch_bwdbwd(const AttnShape& s, int hd, const BwdBwdPtrs& p, int passes, int* status, cudaStream_t stream);
+int launch_bwdbwd(const SinkShape& s, int hd, const BwdBwdPtrs& p, int passes, int* status, cudaStream_t stream);
 
 // Adds up the partial sums that a key pass with s.splits > 1 left in s.sink_part
 // (sink_join.cu): rows of the key tiles that hold a sink of dk and dv, plus the addends.
-int launch_sink_join(const AttnShape& s, int hd, void* dk, void* dv, const void* dk_acc, const void* dv_acc,
+int launch_sink_join(const SinkShape& s, int hd, void* dk, void* dv, const void* dk_acc, const void* dv_acc,
                      cudaStream_t stream);
 
 // fp32 operands on the CUDA cores (f32.cu): same passes, masks, GQA mapping and
@@ -86,9 +86,9 @@ struct F32BwdBwdPtrs {
   float *dd, *bv;
 };
 
-int launch_fwd_f32(const AttnShape& s, int hd, const F32FwdPtrs& p, cudaStream_t stream);
-int launch_bwd_f32(const AttnShape& s, int hd, const F32BwdPtrs& p, cudaStream_t stream);
-int launch_bwdbwd_f32(const AttnShape& s, int hd, const F32BwdBwdPtrs& p, int passes, cudaStream_t stream);
+int launch_fwd_f32(const SinkShape& s, int hd, const F32FwdPtrs& p, cudaStream_t stream);
+int launch_bwd_f32(const SinkShape& s, int hd, const F32BwdPtrs& p, cudaStream_t stream);
+int launch_bwdbwd_f32(const SinkShape& s, int hd, const F32BwdBwdPtrs& p, int passes, cudaStream_t stream);
 
 // LayerNorm over rows of `cols` fp32 values and its backward / double backward
 // (ln_gelu.cu). op 0: forward (out0 = y, out1 = mean, out2 = rstd); op 1: backward

@@ -14,14 +14,14 @@ constexpr int kJoinThreads = 256;
 // One thread per 8 columns of a row of dK or dV. Grid (blocks of rows, key heads, batch).
 template <int HD, bool VL>
 __global__ void __launch_bounds__(kJoinThreads)
-    sink_join_kernel(const AttnShape s, __nv_bfloat16* __restrict__ dk, __nv_bfloat16* __restrict__ dv,
+    sink_join_kernel(const SinkShape s, __nv_bfloat16* __restrict__ dk, __nv_bfloat16* __restrict__ dv,
                      const __nv_bfloat16* dk_acc, const __nv_bfloat16* dv_acc) {
   constexpr int CH = HD / 8;
   const int i = blockIdx.x * kJoinThreads + threadIdx.x;
   const int chunk = i % CH, matrix = (i / CH) & 1, key = i / (2 * CH);
   const int hk = blockIdx.y, b = blockIdx.z;
   SeqRange sr;
-  const AttnShape l = seq_shape<VL>(s, b, &sr);
+  const SinkShape l = seq_shape<VL>(s, b, &sr);
   if (key >= l.Tk) return;
   float v[8] = {};
 #pragma unroll 4
@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kJoinThreads)
 
 }  // namespace
 
-int launch_sink_join(const AttnShape& s, int hd, void* dk, void* dv, const void* dk_acc, const void* dv_acc,
+int launch_sink_join(const SinkShape& s, int hd, void* dk, void* dv, const void* dk_acc, const void* dv_acc,
                      cudaStream_t stream) {
   const int rows = sink_tiles(s) * kBM;
   const dim3 grid((rows * 2 * (hd / 8) + kJoinThreads - 1) / kJoinThreads, s.Hk, s.B);
