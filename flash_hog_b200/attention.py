@@ -105,9 +105,10 @@ def dot_product_attention_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, 
     apply per sequence: "bottom_right" aligns each sequence's own diagonal, the mask of
     the reference's JAX statements for a (qs, ks) pair
     (``flash_hog/_jax_refs/jax_impl.py:104-130``); ``sink_tokens`` are the first keys of
-    each sequence. Each sequence's result equals the
-    dense call on that sequence alone. Computes with bf16 operands (any input dtype;
-    results in the input dtype).
+    each sequence. Each sequence's result equals the dense call on that sequence alone (with
+    sinks, up to rounding for sequences of so few queries that the dense call runs its
+    kernel for single tokens). Computes with bf16 operands (any input dtype; results in the
+    input dtype).
     """
     if query.ndim != 3 or key.ndim != 3 or value.ndim != 3:
         raise ValueError("packed tensors are (total, heads, head_dim)")

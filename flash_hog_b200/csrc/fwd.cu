@@ -477,6 +477,7 @@ int launch_fwd_hd(const SinkShape& s, const FwdPtrs& p, int* status, cudaStream_
 }  // namespace
 
 int launch_fwd(const SinkShape& s, int hd, const FwdPtrs& p, int* status, cudaStream_t stream) {
+  if (fwd_few_applies(s)) return launch_fwd_few(s, hd, p, stream);
   if (hd == 64) return s.cu_q ? launch_fwd_hd<64, true>(s, p, status, stream) : launch_fwd_hd<64, false>(s, p, status, stream);
   if (hd == 128) return s.cu_q ? launch_fwd_hd<128, true>(s, p, status, stream) : launch_fwd_hd<128, false>(s, p, status, stream);
   return kUnsupported;
