@@ -159,7 +159,9 @@ int validate(const fh_attn_dims* d, SinkShape* out, float scale, int causal, boo
   } else {
     out->cu_q = out->cu_k = nullptr;
     out->diag = causal == 2 ? d->seq_k - d->seq_q : 0;
-    if (d->seq_q + out->diag <= d->window) out->sinks = 0;  // the window hides nothing
+    // A window that hides nothing is the mask without sinks, but for the few rows that have
+    // a kernel of their own with them.
+    if (d->seq_q + out->diag <= d->window && static_cast<long long>(d->seq_q) * out->G > kFewRows) out->sinks = 0;
   }
   out->sink_part = static_cast<float*>(d->sink_scratch);
   out->splits = 1;

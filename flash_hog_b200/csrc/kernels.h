@@ -50,7 +50,9 @@ struct BwdBwdPtrs {
 };
 
 int launch_fwd(const SinkShape& s, int hd, const FwdPtrs& p, int* status, cudaStream_t stream);
-// The forward of a few query rows over a window with sinks (fwd_few.cu), where it applies.
+// The forward of a few query rows over a window with sinks (fwd_few.cu), where it applies:
+// up to kFewRows rows, tokens x query heads of a key head.
+constexpr int kFewRows = 16;
 bool fwd_few_applies(const SinkShape& s);
 int launch_fwd_few(const SinkShape& s, int hd, const FwdPtrs& p, cudaStream_t stream);
 int launch_rowdot(const AttnShape& s, int hd, const void* o, const void* dO, float* delta, cudaStream_t stream);

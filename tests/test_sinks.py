@@ -149,6 +149,7 @@ FEW = [  # b, h, hk, tq, tk, causal, window, sinks
     (3, 4, 4, 1, 2000, 2, 300, 4), (2, 8, 2, 1, 5000, 2, 1024, 4), (1, 8, 1, 1, 8192, 2, 4096, 64),
     (2, 2, 2, 5, 900, 2, 100, 3), (1, 4, 2, 4, 333, 2, 17, 40), (1, 8, 1, 1, 40, 2, 7, 9), (300, 1, 1, 1, 90, 2, 16, 1),
     (1, 2, 2, 3, 64, 1, 2, 1), (2, 2, 1, 4, 3, 2, 1, 1), (1, 1, 1, 8, 500, 2, 1, 1), (2, 3, 3, 7, 300, 2, 64, 255),
+    (2, 4, 2, 8, 700, 2, 99, 5), (1, 16, 1, 1, 1000, 2, 2000, 4), (3, 5, 1, 3, 129, 2, 128, 1),
 ]
 
 
@@ -157,7 +158,7 @@ FEW = [  # b, h, hk, tq, tk, causal, window, sinks
 @pytest.mark.parametrize("packed", [False, True])
 @pytest.mark.parametrize("b,h,hk,tq,tk,causal,window,sinks", FEW)
 def test_few_query_rows(b, h, hk, tq, tk, causal, window, sinks, packed, d):
-    """Single tokens and a handful: fp32 products and probabilities, so within the output's
+    """Single tokens and a handful: fp32 sums, probabilities to 2^-17, so within the output's
     rounding (half a step of bf16, 2^-8: it has 8 significant bits) and 2^-13 of the largest
     value (sums of up to 4160 terms near 1e-5 off)."""
     from flash_hog_b200 import _capi
@@ -300,10 +301,10 @@ def test_public_varlen_op():
     for b in range(len(lq)):
         sq, sk = slice(int(cq[b]), int(cq[b + 1])), slice(int(ck[b]), int(ck[b + 1]))
         one = fhb.dot_product_attention(q[sq][None], k[sk][None], v[sk][None], **kw)[0]
-        if lq[b] > 8:
+        if lq[b] > 16:
             assert torch.equal(out[sq], one)
         else:
-            # Alone, few rows run a kernel with fp32 probabilities; the packed batch's rounds them
+            # Alone, few rows run a kernel with finer probabilities; the packed batch's rounds them
             # to bf16 (2^-8 of each), and both round their output (2^-8).
             bound = 2.0 ** -8 * (v[sk].float().abs().amax(0) + 2 * one.float().abs())
             assert ((out[sq].float() - one.float()).abs() <= bound).all()
