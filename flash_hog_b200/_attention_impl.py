@@ -271,7 +271,8 @@ def dot_product_attention_fwd_jvp(mask_type: MaskType, scale: float, res, tangen
     if f32:
         stats = torch.empty((2, b, n, t), dtype=torch.float32, device=q.device)
         _capi.attn_bwdbwd_f32(q, k, v, o, torch.zeros_like(q), tq, tk, tv, lse, None, t_out, None, None, stats[0],
-                              t_lse, stats[1], scale, causal, which=_capi.PASS_QUERY, window=window, **_mask_kw(mask_type))
+                              t_lse, stats[1], scale, causal, which=_capi.PASS_QUERY, window=window,
+                              **_mask_kw(mask_type))
     else:
         # The forward-tangent pass: the query pass at dO = 0, without the products that vanish there.
         _capi.attn_bwdbwd_o(q, k, v, None, None, tq, tk, tv, lse, None, t_out, None, None, None, t_lse, None, scale,

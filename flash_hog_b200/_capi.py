@@ -222,7 +222,10 @@ def _addr(t):
 
 
 def _raw_stream(t: torch.Tensor) -> int:
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
+    index = t.get_device()
+    if index < 0:
+        raise ValueError("flash_hog_b200 runs on CUDA tensors only")
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _strides(t: torch.Tensor) -> FhStrides:
@@ -413,7 +416,8 @@ def attn_fwd_f32(q, k, v, out, lse, scale: float, causal: int, window: int = 0, 
 
 
 @_on_device
-def attn_bwd_f32(q, k, v, o, dO, lse, dq, dk, dv, delta, scale: float, causal: int, window: int = 0, sinks: int = 0) -> None:
+def attn_bwd_f32(q, k, v, o, dO, lse, dq, dk, dv, delta, scale: float, causal: int, window: int = 0,
+                 sinks: int = 0) -> None:
     """``attn_bwd`` with fp32 tensors (``fh_attn_bwd_f32``)."""
     _same_layout(q, o, dO, dq, dtype=_F32)
     _same_layout(k, v, dk, dv, dtype=_F32)

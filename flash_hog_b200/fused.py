@@ -414,8 +414,8 @@ def policy_loss(logits, actions, old_logprobs, advantages, *, ref_logprobs=None,
         raise ValueError("kl_coef must be finite and >= 0")
     if kl_coef > 0.0 and ref_logprobs is None:
         raise ValueError("kl_coef > 0 needs ref_logprobs")
-    if normalizer is not None and not 0.0 < normalizer < float("inf"):
-        raise ValueError("normalizer must be positive and finite")
+    if normalizer is not None and not 2.0 ** -126 <= normalizer < 2.0 ** 128:
+        raise ValueError("normalizer must be positive and finite (a normal fp32 number)")
     if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
         logits = logits.contiguous()
     return _PolicyLoss.apply(logits, _contig(actions.long()), _f32(old_logprobs), _f32(advantages),

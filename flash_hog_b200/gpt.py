@@ -112,6 +112,8 @@ class GPT(nn.Module):
 
     def __init__(self, cfg: GPTConfig, attention: str = "flash", fused: bool | None = None):
         super().__init__()
+        if cfg.sinks and cfg.window is None:
+            raise ValueError("GPTConfig.sinks apply to a window")
         fn = {"flash": dot_product_attention, "naive": naive_attention}[attention]
         fused = attention == "flash" if fused is None else fused
         self.cfg, self.fused = cfg, fused

@@ -161,6 +161,20 @@ def test_shapes_strides_and_index_types():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tables_and_gradients_off_the_vector_alignment(dtype):
+    from flash_hog_b200 import fused
+
+    w = torch.randn(40 * 16 + 1, device="cuda").to(dtype)[1:].view(40, 16).requires_grad_(True)
+    dy = torch.randn(100 * 16 + 1, device="cuda").to(dtype)[1:].view(100, 16)
+    t = torch.randint(0, 40, (100,), device="cuda")
+    y = fused.embedding(t, w, 0.7)
+    _check_lookup(y.detach(), w.detach(), t, 0.7)
+    (dw,) = torch.autograd.grad(y, w, dy)
+    _check_grad(dw, t, dy, 40, 0.7)
+
+
+@pytest.mark.gpu
 def test_module_matches_nn_embedding():
     from flash_hog_b200 import fused
 

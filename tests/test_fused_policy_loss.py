@@ -268,7 +268,7 @@ def test_refusals():
     with pytest.raises(ValueError):
         fused.policy_loss(z[:, :0], a, v, v)
     for kw in (dict(clip_low=-0.1), dict(clip_high=float("nan")), dict(kl_coef=0.1), dict(kl_coef=-1.0),
-               dict(normalizer=0.0), dict(normalizer=float("inf"))):
+               dict(normalizer=0.0), dict(normalizer=1e-40), dict(normalizer=float("inf"))):
         with pytest.raises(ValueError):
             fused.policy_loss(z, a, v, v, **kw)
 

@@ -40,6 +40,11 @@ def test_naive_attention_has_the_window():
         torch.testing.assert_close(got[0, i], want, rtol=1e-5, atol=1e-5)
 
 
+def test_sinks_need_a_window():
+    with pytest.raises(ValueError):
+        GPT(GPTConfig(n_layer=1, d_model=64, n_head=1, d_mlp=64, vocab=50, seq_len=16, sinks=2))
+
+
 def _close(got, want, tol):
     """Relative distance of two lists of gradients, as a whole and each by itself (looser)."""
     num = sum(((a.double() - b.double()) ** 2).sum() for a, b in zip(got, want)).sqrt()

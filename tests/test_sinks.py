@@ -361,6 +361,43 @@ def test_captured_and_replayed():
 
 
 @pytest.mark.gpu
+def test_token_step_captured_and_replayed_on_other_contents():
+    """A server's captured step: keys and values that grow in place, one query."""
+    import flash_hog_b200 as fhb
+
+    x = {n: t.cuda() for n, t in _inputs(3, 8, 2, 1, 600, 64, torch.bfloat16).items()}
+    kw = dict(is_causal=True, causal_alignment="bottom_right", sliding_window_length=128, sink_tokens=4)
+    run = lambda: fhb.dot_product_attention(x["q"], x["k"], x["v"], **kw)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for seed in (31, 32):
+        for n, t in _inputs(3, 8, 2, 1, 600, 64, torch.bfloat16, seed=seed).items():
+            x[n].copy_(t)
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, run())
+
+
+@pytest.mark.gpu
+def test_hidden_keys_are_not_read_by_tokens():
+    """What lies between the sinks and the window (an evicted cache) may hold anything."""
+    import flash_hog_b200 as fhb
+
+    x = {n: t.cuda() for n, t in _inputs(2, 4, 2, 1, 900, 64, torch.bfloat16).items()}
+    kw = dict(is_causal=True, causal_alignment="bottom_right", sliding_window_length=100, sink_tokens=6)
+    want = fhb.dot_product_attention(x["q"], x["k"], x["v"], **kw)
+    x["k"][:, 6:800] = float("nan")
+    x["v"][:, 6:800] = float("inf")
+    assert torch.equal(fhb.dot_product_attention(x["q"], x["k"], x["v"], **kw), want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("d", [64, 128])
 def test_long_sequences_with_few_heads(d):
     """Most of the sink tiles' work lies on few CTAs: 40 query tiles for one key tile of sinks."""
