@@ -206,15 +206,6 @@ def _on_device(f):
     return call
 
 
-def _same_device(t: torch.Tensor, *others) -> None:
-    index = t.get_device()
-    if index < 0:
-        raise ValueError("flash_hog_b200 runs on CUDA tensors only")
-    for x in others:
-        if x is not None and x.get_device() != index:
-            raise ValueError(f"tensors must be on one CUDA device, got {t.device} and {x.device}")
-
-
 # Addresses and streams as plain integers, which ctypes converts by the argtypes: for the
 # small calls, whose time is the host's, building c_void_p objects is a tenth of it.
 def _addr(t):
@@ -541,112 +532,18 @@ def xent_bwd_bwd(z, t, lse, g, s: float, u, gz, gg) -> None:
                                                      _ptr(lse), _ptr(g), float(s), _ptr(u), _ptr(gz), _ptr(gg)))
 
 
-def _embed_args(rows, table, tokens):
-    """(dtype, n, vocab, dim) of (n, dim) rows against a (vocab, dim) table."""
-    _same_device(table, rows, tokens)
-    if table.dim() != 2 or table.dtype not in _GELU_DTYPES or not table.is_contiguous():
-        raise ValueError("an embedding table is a contiguous (vocab, dim) fp32 or bf16 tensor")
-    if tokens.dtype != torch.int64 or not tokens.is_contiguous():
-        raise ValueError("embedding tokens are a contiguous int64 tensor")
-    n, (vocab, dim) = tokens.numel(), table.shape
-    if rows.dtype != table.dtype or not rows.is_contiguous() or rows.numel() != n * dim:
-        raise ValueError("embedding rows are a contiguous (tokens, dim) tensor of the table's dtype")
-    if n >= 2 ** 31 or vocab >= 2 ** 31 - 1:
-        raise ValueError("embedding: fewer than 2^31 tokens and 2^31 - 1 table rows")
-    return _GELU_DTYPES[table.dtype], n, vocab, dim
-
-
-@_on_device
-def embed_fwd(w, tokens, scale: float, y) -> None:
-    """y_i = scale w[t_i]; see fh_embed_fwd."""
-    args = _embed_args(y, w, tokens)
-    _check("fh_embed_fwd", lib().fh_embed_fwd(_raw_stream(w), *args, _addr(w), _addr(tokens), float(scale), _addr(y)))
-
-
-@_on_device
-def embed_bwd(dy, tokens, scale: float, padding_idx: int, dw) -> None:
-    """dw[v] = scale sum_{t_i = v} dy_i; see fh_embed_bwd."""
-    args = _embed_args(dy, dw, tokens)
-    scratch = torch.empty(int(lib().fh_embed_scratch_bytes(args[1], args[3])), dtype=torch.uint8, device=dw.device)
-    _check("fh_embed_bwd", lib().fh_embed_bwd(_raw_stream(dw), *args, _addr(dy), _addr(tokens), float(scale),
-                                             int(padding_idx), _addr(dw), _addr(scratch)))
-
-
-@_on_device
-def embed_bwd_bwd(ddw, tokens, scale: float, padding_idx: int, ddy) -> None:
-    """ddy_i = scale ddw[t_i], 0 for padding; see fh_embed_bwd_bwd."""
-    args = _embed_args(ddy, ddw, tokens)
-    _check("fh_embed_bwd_bwd", lib().fh_embed_bwd_bwd(_raw_stream(ddw), *args, _addr(ddw), _addr(tokens),
-                                                     float(scale), int(padding_idx), _addr(ddy)))
-
-
-@_on_device
-def dropout(x, res, y, seed, subsequence: int, limit: int) -> None:
-    """y = res + keep x / (1 - limit / 65536); see fh_dropout. ``res`` may be None."""
-    _same_device(x, res, y, seed)
-    if seed.dtype is not torch.int64 or seed.numel() != 1:
-        raise ValueError("the dropout seed is an int64 tensor of one element")
-    shape = x.shape
-    for t in (x, y) if res is None else (x, y, res):
-        if t.dtype not in _GELU_DTYPES or not t.is_contiguous() or t.shape != shape:
-            raise ValueError("dropout tensors are contiguous fp32 or bf16 tensors of one shape")
-    _check("fh_dropout", lib().fh_dropout(
-        _raw_stream(x), x.numel(), _GELU_DTYPES[x.dtype], _addr(x), 0 if res is None else _GELU_DTYPES[res.dtype],
-        _addr(res), _GELU_DTYPES[y.dtype], _addr(y), _addr(seed), int(subsequence), int(limit)))
-
-
-def _policy_args(z, actions, *vectors):
-    """(dtype, rows, vocab, ld) of the logits; ``vectors``: fp32 tensors of one entry per row, or None."""
-    _same_device(z, actions, *vectors)
-    if z.dim() != 2 or z.dtype not in _GELU_DTYPES or z.shape[1] < 1 or (z.stride(1) != 1 and z.shape[1] > 1):
-        raise ValueError("policy logits are a (rows, vocab) fp32 or bf16 tensor with unit column stride")
-    rows, vocab = z.shape
-    if actions.dtype != torch.int64 or not actions.is_contiguous() or actions.shape != (rows,):
-        raise ValueError("policy actions are a contiguous int64 vector of one entry per row")
-    for v in vectors:
-        if v is not None and (v.dtype != torch.float32 or not v.is_contiguous() or v.shape != (rows,)):
-            raise ValueError("the policy's per-row inputs are contiguous fp32 vectors of one entry per row")
-    return _GELU_DTYPES[z.dtype], rows, vocab, z.stride(0) if rows > 1 else vocab
-
-
-def policy_stats(z) -> torch.Tensor:
-    """Uninitialised ``stats`` of ``policy_fwd`` for these logits."""
-    return torch.empty(int(lib().fh_policy_stats_floats(z.shape[0], z.shape[1])), dtype=torch.float32, device=z.device)
-
-
-@_on_device
-def policy_fwd(z, actions, old, adv, ref, weights, clip_low: float, clip_high: float, kl_coef: float,
-               normalizer: float, lp, loss, stats) -> None:
-    """Loss, log probabilities and the backward's statistics; see fh_policy_fwd."""
-    args = _policy_args(z, actions, old, adv, ref, weights, lp)
-    _check("fh_policy_fwd", lib().fh_policy_fwd(
-        _raw_stream(z), *args, _addr(z), _addr(actions), _addr(old), _addr(adv), _addr(ref), _addr(weights),
-        float(clip_low), float(clip_high), float(kl_coef), float(normalizer), _addr(lp), _addr(loss), _addr(stats)))
-
-
-@_on_device
-def policy_bwd(z, actions, stats, g, dz) -> None:
-    """dz = g dloss/dz; g a one-element fp32 device tensor."""
-    args = _policy_args(z, actions)
-    _same_device(z, stats, g, dz)
-    if dz.dtype != z.dtype or not dz.is_contiguous() or dz.shape != z.shape:
-        raise ValueError("dz is a contiguous tensor of the logits' shape and dtype")
-    _check("fh_policy_bwd", lib().fh_policy_bwd(_raw_stream(z), *args, _addr(z), _addr(actions), _addr(stats),
-                                               _addr(g), _addr(dz)))
-
-
-@_on_device
-def policy_bwd_bwd(z, actions, stats, g, u, gz, gg) -> None:
-    """Backward's backward given the cotangent u of dz; see fh_policy_bwd_bwd."""
-    args = _policy_args(z, actions, gg)
-    _same_device(z, stats, g, u, gz)
-    for x in (u, gz):
-        if x.dtype != z.dtype or not x.is_contiguous() or x.shape != z.shape:
-            raise ValueError("u and gz are contiguous tensors of the logits' shape and dtype")
-    n = int(lib().fh_policy_scratch_floats(z.shape[0], z.shape[1]))
-    scratch = torch.empty(n, dtype=torch.float32, device=z.device) if n else None
-    _check("fh_policy_bwd_bwd", lib().fh_policy_bwd_bwd(_raw_stream(z), *args, _addr(z), _addr(actions), _addr(stats),
-                                                       _addr(g), _addr(u), _addr(gz), _addr(gg), _addr(scratch)))
+@functools.cache
+def torch_ops():
+    """``_torch_ops``: the autograd nodes of the embedding, dropout and policy loss
+    (``csrc/torch_ops.cpp``), on this process's library."""
+    try:
+        from flash_hog_b200 import _torch_ops
+    except ImportError as e:
+        raise RuntimeError("flash_hog_b200/_torch_ops.so does not load; build it with `python -m flash_hog_b200.build`"
+                           ) from e
+    h = lib()
+    _torch_ops.bind({name: ctypes.cast(getattr(h, name), ctypes.c_void_p).value for name in EXPORTED_SYMBOLS})
+    return _torch_ops
 
 
 def launch_count() -> int:

@@ -1,8 +1,9 @@
 """Build the in-tree CUDA library for sm_100a with nvcc.
 
-``libflashhog_b200.so`` -- the attention kernels and the C ABI declared in
+``libflashhog_b200.so`` -- the kernels and the C ABI declared in
 ``include/flash_hog_b200.h`` -- is written next to this file so it travels with
-the source tree. Object files are cached under ``_build/`` keyed by source and
+the source tree, and so is ``_torch_ops.so``, the autograd nodes of ``fused``'s
+embedding, dropout and policy loss over that ABI (``csrc/torch_ops.cpp``). Object files are cached under ``_build/`` keyed by source and
 header modification times, so an unchanged tree rebuilds in well under a second.
 """
 
@@ -27,6 +28,8 @@ MAIN_SOURCES = ["capi.cu", "fwd.cu", "fwd_few.cu", "bwd.cu", "bwdbwd.cu", "sink_
                 "ln_gelu.cu", "xent.cu", "embed.cu", "dropout.cu", "policy.cu"]
 
 MAIN_LIB = os.path.join(PKG, "libflashhog_b200.so")
+TORCH_OPS_SOURCE = os.path.join(CSRC, "torch_ops.cpp")
+TORCH_OPS_LIB = os.path.join(PKG, "_torch_ops.so")
 
 
 def nvcc() -> str:
@@ -67,11 +70,34 @@ def _link(objs, out):
         raise RuntimeError(f"link of {os.path.basename(out)} failed:\n{res.stdout}\n{res.stderr}")
 
 
+def build_torch_ops() -> None:
+    """Compile ``csrc/torch_ops.cpp`` against torch's headers (host code only)."""
+    header = os.path.join(ROOT, "include", "flash_hog_b200.h")
+    if os.path.exists(TORCH_OPS_LIB) and os.path.getmtime(TORCH_OPS_LIB) >= max(
+            os.path.getmtime(TORCH_OPS_SOURCE), os.path.getmtime(header)):
+        return
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    includes = cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"], os.path.dirname(header)]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *["-isystem" + i for i in includes],
+           TORCH_OPS_SOURCE, "-o", TORCH_OPS_LIB, *["-L" + p for p in cpp_extension.library_paths("cuda")],
+           "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on torch_ops.cpp:\n{res.stdout}\n{res.stderr}")
+
+
 def build(verbose: bool = False) -> None:
-    """Compile every CUDA source of the library for sm_100a and link it."""
+    """Compile every CUDA source of the library for sm_100a and link it; then the torch nodes."""
     srcs = MAIN_SOURCES
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        torch_ops = ex.submit(build_torch_ops)
         objs = dict(zip(srcs, ex.map(lambda s: _compile(s, verbose), srcs)))
+        torch_ops.result()
     _link([objs[s] for s in MAIN_SOURCES], MAIN_LIB)
 
 

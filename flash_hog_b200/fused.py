@@ -34,7 +34,6 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd import forward_ad
 
 from flash_hog_b200 import _capi
 
@@ -184,68 +183,6 @@ def cross_entropy(logits, targets):
     return _CrossEntropy.apply(logits, _contig(targets.long()))
 
 
-def _untracked(*ts) -> bool:
-    """Whether no derivative of a call on ``ts`` will be asked for: the call then goes to
-    the kernel without an autograd node (about 5 us of host time less)."""
-    if forward_ad._current_level >= 0:
-        return False
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
-                return False
-    return True
-
-
-def _embedding_run(w, tokens, scale, padding_idx, adjoint):
-    y = torch.empty((*tokens.shape, w.shape[1]), dtype=w.dtype, device=w.device)
-    if adjoint:
-        _capi.embed_bwd_bwd(w, tokens, scale, padding_idx, y)
-    else:
-        _capi.embed_fwd(w, tokens, scale, y)
-    return y
-
-
-def _embedding_bwd_run(dy, tokens, vocab, scale, padding_idx):
-    dy = _contig(dy)
-    dw = torch.empty((vocab, dy.shape[-1]), dtype=dy.dtype, device=dy.device)
-    _capi.embed_bwd(dy, tokens, scale, padding_idx, dw)
-    return dw
-
-
-class _Embedding(torch.autograd.Function):
-    """scale W[t]; with ``adjoint``, the derivative of ``_EmbeddingBwd`` (zero rows for
-    padding and for tokens outside the table). Linear in W: its backward is
-    ``_EmbeddingBwd``, whose backward is this one again, to any order."""
-
-    @staticmethod
-    def forward(ctx, w, tokens, scale, padding_idx, adjoint):
-        ctx.save_for_backward(tokens)
-        ctx.args = w.shape[0], scale, padding_idx
-        return _embedding_run(w, tokens, scale, padding_idx, adjoint)
-
-    @staticmethod
-    def backward(ctx, dy):
-        (tokens,) = ctx.saved_tensors
-        grad = _embedding_bwd_run if _untracked(dy) else _EmbeddingBwd.apply
-        return grad(dy, tokens, *ctx.args), None, None, None, None
-
-
-class _EmbeddingBwd(torch.autograd.Function):
-    """dW from dy by sorted tokens, every row written."""
-
-    @staticmethod
-    def forward(ctx, dy, tokens, vocab, scale, padding_idx):
-        ctx.save_for_backward(tokens)
-        ctx.args = scale, padding_idx
-        return _embedding_bwd_run(dy, tokens, vocab, scale, padding_idx)
-
-    @staticmethod
-    def backward(ctx, ddw):
-        (tokens,) = ctx.saved_tensors
-        lookup = _embedding_run if _untracked(ddw) else _Embedding.apply
-        return lookup(_contig(ddw), tokens, *ctx.args, True), None, None, None, None
-
-
 def embedding(tokens, weight, scale: float = 1.0, padding_idx: int | None = None):
     """``scale * weight[tokens]`` for integer ``tokens`` of any shape and a (vocab, dim)
     fp32 or bf16 ``weight``, in the weight's dtype; differentiable to any order.
@@ -254,16 +191,7 @@ def embedding(tokens, weight, scale: float = 1.0, padding_idx: int | None = None
     run) and is zero for ``padding_idx``. A token outside [0, vocab) gives a row of NaN
     and no gradient.
     """
-    if tokens.dtype not in (torch.int64, torch.int32):
-        raise ValueError(f"embedding tokens are int64 or int32, got {tokens.dtype}")
-    if weight.dim() != 2 or weight.dtype not in (torch.float32, torch.bfloat16) or 0 in weight.shape:
-        raise ValueError("the embedding weight is a non-empty (vocab, dim) fp32 or bf16 tensor")
-    if padding_idx is None:
-        padding_idx = -1
-    elif not 0 <= padding_idx < weight.shape[0]:
-        raise ValueError(f"padding_idx must be in [0, {weight.shape[0]}), got {padding_idx}")
-    lookup = _embedding_run if _untracked(weight) else _Embedding.apply
-    return lookup(_contig(weight), _contig(tokens.long()), float(scale), int(padding_idx), False)
+    return _capi.torch_ops().embedding(tokens, weight, scale, padding_idx)
 
 
 class Embedding(nn.Embedding):
@@ -281,34 +209,6 @@ class Embedding(nn.Embedding):
         return embedding(tokens, self.weight, self.scale, self.padding_idx)
 
 
-def _dropout_run(x, residual, seed, subsequence, limit, dtype):
-    y = torch.empty(x.shape, dtype=dtype, device=x.device)
-    _capi.dropout(x, residual, y, seed, subsequence, limit)
-    return y
-
-
-class _Dropout(torch.autograd.Function):
-    """residual + keep x / (1 - p) in ``dtype``. Linear in x: its backward is itself on dy,
-    with the mask drawn again from the saved seed, to any order."""
-
-    @staticmethod
-    def forward(ctx, x, residual, seed, subsequence, limit, dtype):
-        ctx.save_for_backward(seed)
-        ctx.args = subsequence, limit, x.dtype
-        ctx.residual_dtype = None if residual is None else residual.dtype
-        return _dropout_run(x, residual, seed, subsequence, limit, dtype)
-
-    @staticmethod
-    def backward(ctx, dy):
-        (seed,) = ctx.saved_tensors
-        dx = dres = None
-        if ctx.needs_input_grad[0]:
-            dx = (_dropout_run if _untracked(dy) else _Dropout.apply)(_contig(dy), None, seed, *ctx.args)
-        if ctx.needs_input_grad[1]:
-            dres = dy.to(ctx.residual_dtype)
-        return dx, dres, None, None, None, None
-
-
 def dropout(x, p: float, seed, *, subsequence: int = 0, residual=None):
     """``residual + keep * x / (1 - p)`` (without ``residual``: 0) for fp32 or bf16 tensors,
     differentiable to any order; in ``x``'s dtype, or with a residual in the promoted one.
@@ -321,75 +221,7 @@ def dropout(x, p: float, seed, *, subsequence: int = 0, residual=None):
     ``subsequence`` in [0, 2^32) separates calls that share a seed (one per layer). ``p``
     in [0, 1] is rounded to a multiple of 2^-16; at p = 1 everything is dropped.
     """
-    if not 0.0 <= p <= 1.0:
-        raise ValueError(f"dropout p must be in [0, 1], got {p}")
-    if not 0 <= subsequence < 2 ** 32:
-        raise ValueError(f"subsequence must be in [0, 2^32), got {subsequence}")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"the residual must have x's shape, got {tuple(residual.shape)} and {tuple(x.shape)}")
-    for t in (x, residual):
-        if t is not None and t.dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError(f"dropout takes fp32 or bf16 tensors, got {t.dtype}")
-    dtype = x.dtype if residual is None else torch.promote_types(x.dtype, residual.dtype)
-    run = _dropout_run if _untracked(x, residual) else _Dropout.apply
-    return run(_contig(x), None if residual is None else _contig(residual), seed, int(subsequence), round(p * 65536),
-               dtype)
-
-
-def _f32(t):
-    """``t`` as a contiguous fp32 constant."""
-    if t.requires_grad:
-        t = t.detach()
-    return _contig(t if t.dtype is torch.float32 else t.float())
-
-
-def _policy_bwd_run(z, actions, stats, g):
-    dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-    _capi.policy_bwd(z, actions, stats, _f32(g), dz)
-    return dz
-
-
-class _PolicyLossBwd(torch.autograd.Function):
-    """dz = g dloss/dz; its backward is the double backward."""
-
-    @staticmethod
-    def forward(ctx, z, actions, stats, g):
-        g32 = _f32(g)
-        dz = _policy_bwd_run(z, actions, stats, g32)
-        ctx.save_for_backward(z, actions, stats, g32)
-        ctx.g_shape, ctx.g_dtype = g.shape, g.dtype
-        return dz
-
-    @staticmethod
-    def backward(ctx, u):
-        z, actions, stats, g32 = ctx.saved_tensors
-        if any(ctx.needs_input_grad) and torch.is_grad_enabled():
-            raise NotImplementedError("third-order derivatives of the fused policy loss are not supported")
-        u = _contig(u.to(z.dtype))
-        gz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        gg = torch.empty(z.shape[0], dtype=torch.float32, device=z.device)
-        _capi.policy_bwd_bwd(z, actions, stats, g32, u, gz, gg)
-        return gz, None, None, gg.sum().to(ctx.g_dtype).reshape(ctx.g_shape)
-
-
-class _PolicyLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, actions, old, adv, ref, weights, clip_low, clip_high, kl_coef, normalizer):
-        rows = z.shape[0]
-        lp = torch.empty(rows, dtype=torch.float32, device=z.device)
-        loss = torch.empty((), dtype=torch.float32, device=z.device)
-        stats = _capi.policy_stats(z)
-        _capi.policy_fwd(z, actions, old, adv, ref, weights, clip_low, clip_high, kl_coef, normalizer, lp, loss, stats)
-        ctx.save_for_backward(z, actions, stats)
-        ctx.mark_non_differentiable(lp)
-        return loss, lp
-
-    @staticmethod
-    def backward(ctx, g, _g_lp):
-        z, actions, stats = ctx.saved_tensors
-        # Under create_graph dz depends on z, whether or not g is tracked.
-        grad = _PolicyLossBwd.apply if torch.is_grad_enabled() else _policy_bwd_run
-        return (grad(z, actions, stats, g),) + (None,) * 9
+    return _capi.torch_ops().dropout(x, p, seed, subsequence, residual)
 
 
 def policy_loss(logits, actions, old_logprobs, advantages, *, ref_logprobs=None, weights=None, clip_low: float = 0.2,
@@ -406,22 +238,8 @@ def policy_loss(logits, actions, old_logprobs, advantages, *, ref_logprobs=None,
     constant. ``logprobs`` (fp32, detached) are the lp, 0 in rows of weight 0.
     An action outside [0, vocab) in a weighted row gives NaN.
     """
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.shape[1] == 0:
-        raise ValueError("policy_loss takes (rows, vocab) fp32 or bf16 logits")
-    if not (clip_low >= 0.0 and clip_high >= 0.0):
-        raise ValueError("clip_low and clip_high must be >= 0")
-    if not 0.0 <= kl_coef < float("inf"):
-        raise ValueError("kl_coef must be finite and >= 0")
-    if kl_coef > 0.0 and ref_logprobs is None:
-        raise ValueError("kl_coef > 0 needs ref_logprobs")
-    if normalizer is not None and not 2.0 ** -126 <= normalizer < 2.0 ** 128:
-        raise ValueError("normalizer must be positive and finite (a normal fp32 number)")
-    if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
-        logits = logits.contiguous()
-    return _PolicyLoss.apply(logits, _contig(actions.long()), _f32(old_logprobs), _f32(advantages),
-                             _f32(ref_logprobs) if kl_coef > 0.0 else None, None if weights is None else _f32(weights),
-                             float(clip_low), float(clip_high), float(kl_coef),
-                             0.0 if normalizer is None else float(normalizer))
+    return _capi.torch_ops().policy_loss(logits, actions, old_logprobs, advantages, ref_logprobs, weights, clip_low,
+                                         clip_high, kl_coef, normalizer)
 
 
 class _SumOfSquares(torch.autograd.Function):

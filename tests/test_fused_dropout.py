@@ -191,6 +191,44 @@ def test_refusals_on_the_device():
             fused.dropout(x, 0.5, seed)
 
 
+@pytest.mark.gpu
+def test_library_errors_reach_the_caller_from_both_passes(monkeypatch):
+    """A status from the library (injected on the host) is a FlashHogError with its name, in the
+    forward and out of the engine's threads."""
+    from flash_hog_b200 import fused
+    from flash_hog_b200._capi import FlashHogError
+
+    x = torch.randn(8, device="cuda", requires_grad=True)
+    w = torch.randn(4, 4, device="cuda", requires_grad=True)
+    t = torch.zeros(2, dtype=torch.long, device="cuda")
+    monkeypatch.setenv("FLASH_HOG_B200_INJECT_ERROR", "fh_dropout,fh_embed_bwd")
+    with pytest.raises(FlashHogError, match="FH_ERR_INJECTED") as e:
+        fused.dropout(x, 0.5, _seed(1))
+    assert e.value.entry == "fh_dropout" and e.value.status == 5
+    y = fused.embedding(t, w)
+    with pytest.raises(FlashHogError, match="fh_embed_bwd"):
+        y.sum().backward()
+    monkeypatch.delenv("FLASH_HOG_B200_INJECT_ERROR")
+    y = fused.embedding(t, w)
+    y.sum().backward()
+    assert w.grad[0].tolist() == [2.0] * 4
+
+
+@pytest.mark.gpu
+def test_transforms_are_refused():
+    from flash_hog_b200 import fused
+
+    x, seed = torch.randn(3, 8, device="cuda"), _seed(1)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.vmap(lambda v: fused.dropout(v, 0.5, seed))(x)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.grad(lambda v: fused.dropout(v, 0.5, seed).sum())(x)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            fused.dropout(dual, 0.5, seed)
+
+
 def test_refusals():
     from flash_hog_b200 import fused
 
