@@ -100,15 +100,16 @@ def _is_causal(mask) -> bool:
     return _mask_args(mask)[0] != 0
 
 
-def transformed(*ts) -> bool:
-    """Whether forward-mode differentiation or a ``torch.func`` transform is at work on ``ts``."""
-    return forward_ad._current_level >= 0 or any(torch._C._functorch.is_functorch_wrapped_tensor(t) for t in ts)
+def transformed() -> bool:
+    """Whether forward-mode differentiation or a ``torch.func`` transform is at work. (Under a
+    transform autograd Functions need its rules even for tensors that it does not wrap.)"""
+    return forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
 
 
 def untracked(*ts) -> bool:
     """Whether no derivative of a call on ``ts`` will be asked for, and no transform is at
-    work on them: the kernel is called without an autograd node (about 20 us of host time)."""
-    return not transformed(*ts) and (not torch.is_grad_enabled() or not any(t.requires_grad for t in ts))
+    work: the kernel is called without an autograd node (about 20 us of host time)."""
+    return not transformed() and (not torch.is_grad_enabled() or not any(t.requires_grad for t in ts))
 
 
 FP32_POLICY_ENV = "FLASH_HOG_B200_FP32"

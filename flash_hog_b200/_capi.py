@@ -534,8 +534,8 @@ def xent_bwd_bwd(z, t, lse, g, s: float, u, gz, gg) -> None:
 
 @functools.cache
 def torch_ops():
-    """``_torch_ops``: the autograd nodes of the embedding, dropout and policy loss
-    (``csrc/torch_ops.cpp``), on this process's library."""
+    """``_torch_ops``: the autograd nodes of dense attention, the embedding, dropout and policy
+    loss (``csrc/torch_ops.cpp``), on this process's library."""
     try:
         from flash_hog_b200 import _torch_ops
     except ImportError as e:

@@ -23,6 +23,9 @@ Hessian-vector products -- runs fwd, bwd, the forward jvp (the double
 backward's query pass at dO = 0) and the backward's jvp (double backward plus
 first-order backward, ``fh_attn_jvp_bwd``) on the kernels.
 
+Plain calls -- no transform or forward mode at work -- of dense attention take the same
+three rules as C++ nodes (``csrc/torch_ops.cpp``), which cost a third of the host time.
+
 Both Functions, and ``flash_bwdbwd``, also have batching rules for
 ``torch.func.vmap``: the vmapped axis is folded into the batch axis and the
 kernels run once, the rule the reference gives its double backward
@@ -34,6 +37,7 @@ from __future__ import annotations
 import torch
 
 from flash_hog_b200 import _attention_impl as attn_impl
+from flash_hog_b200 import _capi
 from flash_hog_b200._attention_impl import MaskType, PackedSequences, SlidingWindow
 
 
@@ -81,11 +85,13 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
     # The fp32 policy is decided once here and kept with the residuals: the backward,
     # double backward and forward-mode rules of this graph all follow it.
     policy = attn_impl.fp32_policy()
-    if attn_impl.untracked(query, key, value):
-        result = attn_impl.cuda_dot_product_attention(query, key, value, mask_type=mask_type, scale=float(scale),
-                                                      policy=policy)
+    if query.is_cuda and not attn_impl.transformed():
+        causal, window = attn_impl._mask_args(mask_type)
+        result = _capi.torch_ops().attention(query, key, value, causal, window,
+                                             attn_impl._mask_kw(mask_type).get("sinks", 0), scale,
+                                             attn_impl._is_f32(query, policy))
     else:
-        result, _ = _function(_Plain, query, key, value).apply(query, key, value, mask_type, float(scale), policy)
+        result, _ = _DotProductAttention.apply(query, key, value, mask_type, float(scale), policy)
     if unbatched:
         result = result.squeeze(0)
     return result
@@ -116,7 +122,7 @@ def dot_product_attention_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, 
         scale = query.shape[-1] ** -0.5
     mask = _mask_of(is_causal, causal_alignment, sliding_window_length, sink_tokens)
     packed = PackedSequences(mask, cu_seqlens_q, cu_seqlens_k, int(max_seqlen_q), int(max_seqlen_k))
-    result, _ = _function(_Plain, query, key, value).apply(query.unsqueeze(0), key.unsqueeze(0), value.unsqueeze(0),
+    result, _ = _function(_Plain).apply(query.unsqueeze(0), key.unsqueeze(0), value.unsqueeze(0),
                                                            packed, float(scale), "bf16")
     return result.squeeze(0)
 
@@ -126,17 +132,37 @@ def _no_packed_vmap(mask_type):
         raise NotImplementedError("packed variable-length batches are not vmapped: pack the sequences instead")
 
 
-def _function(plain, *ts):
+def _node_mask(causal, window, sinks):
+    return SlidingWindow(MaskType(causal), window, sinks) if window else MaskType(causal)
+
+
+def _transformed_backward(tensors, causal, window, sinks, scale, f32):
+    """The backward of a plain dense call that is batched or differentiated by a transform
+    (``vmap`` over ``torch.autograd.grad``, say), through the Function that has the rules; ``tensors`` are
+    (q, k, v, L, O, dO)."""
+    return _DotProductAttentionBwd.apply(*tensors, _node_mask(causal, window, sinks), scale, "fp32" if f32 else "bf16")
+
+
+def _transformed_double(tensors, causal, window, sinks, scale, f32):
+    """The same for the double backward; ``tensors`` are (q, k, v, L, O, dO, ddQ, ddK, ddV)."""
+    query, key, value, activation, out, g, *dd = tensors
+    (dq2, dk2, dv2, _, _), ddo = attn_impl.dot_product_attention_bwd_rule_bwd_rule(
+        mask_type=_node_mask(causal, window, sinks), scale=scale, res=(query, key, value, out, activation, g), g=dd,
+        policy="fp32" if f32 else "bf16")
+    return dq2, dk2, dv2, ddo
+
+
+def _function(plain):
     """``plain`` (one of the two Functions at the end), or under a transform the Function
     that it stands for, which has the transforms' rules."""
-    return plain.stands_for if attn_impl.transformed(*ts) else plain
+    return plain.stands_for if attn_impl.transformed() else plain
 
 
-def _plain_backward(g) -> bool:
+def _plain_backward() -> bool:
     """Whether a backward runs for its values alone: no graph of it is being built, and no
     forward-mode or ``torch.func`` transform is differentiating or batching it. It then
     calls the rule itself instead of an autograd node (about 30 us of host time less)."""
-    return not torch.is_grad_enabled() and not attn_impl.transformed(g)
+    return not torch.is_grad_enabled() and not attn_impl.transformed()
 
 
 class _DotProductAttention(torch.autograd.Function):
@@ -164,12 +190,12 @@ class _DotProductAttention(torch.autograd.Function):
         if g is None:
             return None, None, None, None, None, None
         query, key, value, activation, out = ctx.saved_tensors
-        if _plain_backward(g):
+        if _plain_backward():
             dq, dk, dv = attn_impl.dot_product_attention_bwd_rule(
                 mask_type=ctx.mask_type, scale=ctx.scale, res=(query, key, value, activation, out), g=g,
                 policy=ctx.policy)
         else:
-            dq, dk, dv = _function(_PlainBwd, query, key, value, g).apply(query, key, value, activation, out, g,
+            dq, dk, dv = _function(_PlainBwd).apply(query, key, value, activation, out, g,
                                                                           ctx.mask_type, ctx.scale, ctx.policy)
         return dq, dk, dv, None, None, None
 

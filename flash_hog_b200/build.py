@@ -2,8 +2,9 @@
 
 ``libflashhog_b200.so`` -- the kernels and the C ABI declared in
 ``include/flash_hog_b200.h`` -- is written next to this file so it travels with
-the source tree, and so is ``_torch_ops.so``, the autograd nodes of ``fused``'s
-embedding, dropout and policy loss over that ABI (``csrc/torch_ops.cpp``). Object files are cached under ``_build/`` keyed by source and
+the source tree, and so is ``_torch_ops.so``, the autograd nodes of dense
+attention and of ``fused``'s embedding, dropout and policy loss over that ABI
+(``csrc/torch_ops.cpp``). Object files are cached under ``_build/`` keyed by source and
 header modification times, so an unchanged tree rebuilds in well under a second.
 """
 
