@@ -106,6 +106,17 @@ __device__ __forceinline__ float2 exp2_fma2(float2 x) {
   return r;
 }
 
+// The larger of two scores. NAN_OUT: NaN if either is (at the same cost), so that the row's
+// maximum, and with it every column of the row, becomes NaN: exp2_fma2 makes a large finite
+// number of one NaN column.
+template <bool NAN_OUT>
+__device__ __forceinline__ float score_max(float a, float b) {
+  if constexpr (!NAN_OUT) return fmaxf(a, b);
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
 // All lanes of the warp have finished their TMEM accesses; one lane arrives.
 __device__ __forceinline__ void fwd_warp_arrive(uint64_t* bar) {
   tc_fence_before();
@@ -353,17 +364,17 @@ __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
 #pragma unroll
       for (int c = 0; c < 8; ++c) mx[c] = __uint_as_float(v[c]);
 #pragma unroll
-      for (int i = 8; i < BN; ++i) mx[i & 7] = fmaxf(mx[i & 7], __uint_as_float(v[i]));
+      for (int i = 8; i < BN; ++i) mx[i & 7] = score_max<SNK>(mx[i & 7], __uint_as_float(v[i]));
 #pragma unroll
       for (int c = 4; c > 0; c >>= 1)
 #pragma unroll
-        for (int k = 0; k < c; ++k) mx[k] = fmaxf(mx[k], mx[k + c]);
+        for (int k = 0; k < c; ++k) mx[k] = score_max<SNK>(mx[k], mx[k + c]);
       const float tmax = mx[0] * sc2;  // log2 domain
-      const float m_new = fmaxf(m_used, tmax);
+      const float m_new = score_max<SNK>(m_used, tmax);
       float f = 1.f;  // rescale factor of O and l, applied before this tile's P is added
       if (j == 0) {
         m_used = m_new;
-      } else if (m_new > m_used + kRescaleLog2) {
+      } else if (SNK ? !(m_new <= m_used + kRescaleLog2) : m_new > m_used + kRescaleLog2) {  // NaN: also
         f = ex2(m_used - m_new);
         m_used = m_new;
       }

@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) fwd_few_kernel(const FewArgs a
       sum += cl[c] * f;
     }
     const int t = r / sh.G, h = hk * sh.G + r % sh.G;
-    a.o[q_row(sh, sr, t, h) + d] = __float2bfloat16_rn(sum > 0.f ? x / sum : 0.f);  // no visible key: 0
+    a.o[q_row(sh, sr, t, h) + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : x / sum);  // no visible key: 0
     if (d == 0) a.lse[q_stat(sh, sr, t, h)] = (to + log2f(sum)) * kLn2;
   }
   if (a.splits > 1) few_cluster_sync();  // the others have read this CTA's share

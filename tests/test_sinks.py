@@ -398,6 +398,34 @@ def test_hidden_keys_are_not_read_by_tokens():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tq", [1, 3, 40])
+def test_nan_is_not_hidden(tq, dtype):
+    """NaN in a query reaches its own row alone; in a visible key, the rows that see it."""
+    import flash_hog_b200 as fhb
+
+    x = {n: t.cuda() for n, t in _inputs(2, 4, 2, tq, 300, 64, dtype).items()}
+    kw = dict(is_causal=True, causal_alignment="bottom_right", sliding_window_length=100, sink_tokens=6)
+    want = fhb.dot_product_attention(x["q"], x["k"], x["v"], **kw)
+    q = x["q"].clone()
+    q[1, -1, 2] = float("nan")
+    got = fhb.dot_product_attention(q, x["k"], x["v"], **kw)
+    assert got[1, -1, 2].isnan().all()
+    got[1, -1, 2] = want[1, -1, 2]
+    # When a warp rescales may change with a row of it: half a step of the result on each side.
+    near = dict(rtol=2 * torch.finfo(dtype).eps, atol=2 * torch.finfo(dtype).eps * want.abs().max().item())
+    torch.testing.assert_close(got, want, **near)
+    for t in ("k", "v"):
+        bad = {**x, t: x[t].clone()}
+        bad[t][0, 3, 1] = float("nan")  # a sink of heads 2 and 3
+        got = fhb.dot_product_attention(bad["q"], bad["k"], bad["v"], **kw)
+        hit = got[0, :, 2:].isnan()
+        assert hit.all() if t == "k" else hit.any(-1).all()
+        torch.testing.assert_close(got[1], want[1], **near)
+        torch.testing.assert_close(got[0, :, :2], want[0, :, :2], **near)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("d", [64, 128])
 def test_long_sequences_with_few_heads(d):
     """Most of the sink tiles' work lies on few CTAs: 40 query tiles for one key tile of sinks."""
