@@ -578,11 +578,16 @@ int fh_xent_bwd_bwd(void* stream, int dtype, int rows, int vocab, long long ld, 
 // Embedding, dropout and the clipped policy loss
 // ------------------------------------------------------------------------------------
 
+// Rows and columns that the embedding and the policy loss count in 32 bits, with room for a
+// block's stride past the end.
+constexpr int kMostRows = 0x7fffffff - 1024;
+
 static int embed_check(int dtype, int n, int vocab, int dim, const void* x, const long long* tokens, const void* y) {
   g_last_error[0] = 0;
-  if (n < 0 || vocab < 1 || vocab == 0x7fffffff || dim < 1 || dim > (1 << 20) || (dtype != 0 && dtype != 1))
+  if (n < 0 || n > kMostRows || vocab < 1 || vocab == 0x7fffffff || dim < 1 || dim > (1 << 20) ||
+      (dtype != 0 && dtype != 1))
     return fail(FH_ERR_INVALID_ARGUMENT,
-                "embed: n >= 0, vocab in [1, 2^31 - 2], dim in [1, 2^20], dtype 0 (fp32) or 1 (bf16)");
+                "embed: n in [0, 2^31 - 1025], vocab in [1, 2^31 - 2], dim in [1, 2^20], dtype 0 (fp32) or 1 (bf16)");
   if (n > 0 && (!x || !tokens || !y)) return fail(FH_ERR_INVALID_ARGUMENT, "embed: a tensor pointer is NULL");
   return kOk;
 }
@@ -629,7 +634,8 @@ int fh_dropout(void* stream, long long n, int x_dtype, const void* x, int res_dt
   if (injected("fh_dropout")) return FH_ERR_INJECTED;
   g_last_error[0] = 0;
   auto dtype_ok = [](int d) { return d == 0 || d == 1; };
-  if (n < 0 || n > (1ll << 42) || !dtype_ok(x_dtype) || !dtype_ok(y_dtype) || (res && !dtype_ok(res_dtype)) || limit < 0 || limit > 65536)
+  if (n < 0 || n > (1ll << 42) || !dtype_ok(x_dtype) || !dtype_ok(y_dtype) || (res && !dtype_ok(res_dtype)) ||
+      limit < 0 || limit > 65536)
     return fail(FH_ERR_INVALID_ARGUMENT, "dropout: n in [0, 2^42], dtypes 0 (fp32) or 1 (bf16), limit in [0, 65536]");
   if (res && y_dtype != (x_dtype & res_dtype))
     return fail(FH_ERR_INVALID_ARGUMENT, "dropout: with a residual y is bf16 where both inputs are, else fp32");
@@ -643,11 +649,16 @@ int fh_dropout(void* stream, long long n, int x_dtype, const void* x, int res_dt
                         static_cast<unsigned>(limit), factor, st);
 }
 
+static bool policy_sizes_ok(int rows, int vocab) {
+  return rows >= 0 && rows <= kMostRows && vocab >= 1 && vocab <= kMostRows;
+}
+
 static int policy_check(int dtype, int rows, int vocab, long long ld, const void* z, const long long* actions,
                         const float* stats) {
   g_last_error[0] = 0;
-  if (rows < 0 || vocab < 1 || ld < vocab || (dtype != 0 && dtype != 1))
-    return fail(FH_ERR_INVALID_ARGUMENT, "policy: rows >= 0, vocab >= 1, ld >= vocab, dtype 0 (fp32) or 1 (bf16)");
+  if (!policy_sizes_ok(rows, vocab) || ld < vocab || (dtype != 0 && dtype != 1))
+    return fail(FH_ERR_INVALID_ARGUMENT,
+                "policy: rows in [0, 2^31 - 1025], vocab in [1, 2^31 - 1025], ld >= vocab, dtype 0 (fp32) or 1 (bf16)");
   if (!all_aligned(stats) || (rows > 0 && (!z || !actions)))
     return fail(FH_ERR_INVALID_ARGUMENT, "policy: logits, actions and (16-byte aligned) stats are required");
   return kOk;
@@ -655,13 +666,13 @@ static int policy_check(int dtype, int rows, int vocab, long long ld, const void
 
 long long fh_policy_stats_floats(int rows, int vocab) {
   g_last_error[0] = 0;
-  if (rows < 0 || vocab < 1) return -1;
+  if (!policy_sizes_ok(rows, vocab)) return -1;
   return policy_stats_floats(rows, vocab);
 }
 
 long long fh_policy_scratch_floats(int rows, int vocab) {
   g_last_error[0] = 0;
-  if (rows < 0 || vocab < 1) return -1;
+  if (!policy_sizes_ok(rows, vocab)) return -1;
   return policy_scratch_floats(rows, vocab);
 }
 

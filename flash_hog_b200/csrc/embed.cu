@@ -13,7 +13,7 @@
 // than rows, and to add up the rows of equal tokens in an order that does not depend on
 // the run (no floating-point atomics). Three launches:
 //   1. One cluster of CTAs sorts (token, position) stably: a radix sort, least significant
-//      digit first, over two or three digits of at most 10 bits. The digit counts of its
+//      digit first, over one to four digits of at most 10 bits. The digit counts of its
 //      CTAs meet in distributed shared memory, so a pass needs cluster barriers only. The
 //      other clusters of the same launch fill dW with zeros meanwhile: that is most of the
 //      gradient's bytes at the sizes of a training step, and it hides the sort.

@@ -82,7 +82,9 @@ struct PolicyStats {
 
 constexpr int kFinishThreads = 128;
 
-__host__ __device__ inline int finish_blocks(int rows) { return rows > 0 ? (rows + kFinishThreads - 1) / kFinishThreads : 1; }
+__host__ __device__ inline int finish_blocks(int rows) {
+  return rows > 0 ? (rows + kFinishThreads - 1) / kFinishThreads : 1;
+}
 
 // Stretches that a row's columns are cut into: with few rows, as many as it takes to give
 // every SM four CTAs, but none shorter than 4096 columns (7 x 131072 fp32: the sums take
@@ -461,8 +463,8 @@ __global__ void __launch_bounds__(kPolThreads) policy_dots_kernel(PolicyArgs a, 
   if (wk.t == 0) part[static_cast<size_t>(r) * splits + wk.stretch] = static_cast<float>(dot);
 }
 
-// The dot product <p, u> of the row comes from `part` (policy_dots_kernel) or, for whole rows, is formed here: the second
-// reading of z and u then comes from L2.
+// The dot product <p, u> of the row comes from `part` (policy_dots_kernel) or, for whole rows,
+// is formed here: the second reading of z and u then comes from L2.
 template <typename T, int NT>
 __global__ void __launch_bounds__(kPolThreads)
     policy_bwd_bwd_kernel(PolicyArgs a, int splits, const float* __restrict__ part, const float* __restrict__ g,

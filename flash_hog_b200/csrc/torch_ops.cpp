@@ -170,8 +170,8 @@ Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, c10::
   const int64_t vocab = weight.size(0), padding = padding_idx.value_or(-1);
   TORCH_CHECK_VALUE(!padding_idx || (padding >= 0 && padding < vocab), "padding_idx must be in [0, ", vocab, "), got ",
                     padding);
-  TORCH_CHECK_VALUE(tokens.numel() < (1ll << 31) && vocab < (1ll << 31) - 1 && weight.size(1) <= (1 << 20),
-                    "embedding: fewer than 2^31 tokens and 2^31 - 1 table rows of at most 2^20 elements");
+  TORCH_CHECK_VALUE(tokens.numel() < (1ll << 31) - 1024 && vocab < (1ll << 31) - 1 && weight.size(1) <= (1 << 20),
+                    "embedding: fewer than 2^31 - 1024 tokens and 2^31 - 1 table rows of at most 2^20 elements");
   same_device(weight, {&tokens});
   return EmbedLookup::apply(weight.contiguous(), tokens.to(at::kLong).contiguous(), scale, padding, false);
 }
@@ -323,8 +323,8 @@ std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& actio
                                     *normalizer <= std::numeric_limits<float>::max()),
                     "normalizer must be positive and finite (a normal fp32 number)");
   const int64_t rows = logits.size(0);
-  TORCH_CHECK_VALUE(rows < (1ll << 31) && logits.size(1) < (1ll << 31),
-                    "policy_loss: fewer than 2^31 rows and columns");
+  TORCH_CHECK_VALUE(rows < (1ll << 31) - 1024 && logits.size(1) < (1ll << 31) - 1024,
+                    "policy_loss: fewer than 2^31 - 1024 rows and columns");
   TORCH_CHECK_VALUE(!actions.is_floating_point() && actions.dim() == 1 && actions.size(0) == rows,
                     "policy actions are an integer vector of one entry per row");
   same_device(logits, {&actions, &old_logprobs, &advantages});

@@ -327,7 +327,8 @@ int fh_xent_bwd_bwd(void* stream, int dtype, int rows, int vocab, long long ld, 
                     const float* lse, const float* g, float s, const void* u, void* gz, float* gg);
 
 /* Embedding of the same model (no counterpart in the reference): a contiguous (vocab,
- * dim) table w, dtype 0 = fp32, 1 = bf16, and n int64 tokens. Sums and the scaling are
+ * dim) table w, dtype 0 = fp32, 1 = bf16, and n int64 tokens; n up to
+ * 2^31 - 1025, vocab to 2^31 - 2, dim to 2^20. Sums and the scaling are
  * fp32, rounded once to the table's type.
  *  - fh_embed_fwd: y_i = scale w[t_i], (n, dim); a token outside [0, vocab) gives a row
  *    of NaN.
@@ -356,8 +357,8 @@ int fh_embed_bwd_bwd(void* stream, int dtype, int n, int vocab, int dim, const v
 int fh_dropout(void* stream, long long n, int x_dtype, const void* x, int res_dtype, const void* res, int y_dtype,
                void* y, const long long* seed, unsigned int subsequence, int limit);
 
-/* Clipped policy loss with a KL term over logits as in fh_xent_* (rows, vocab, ld, dtype).
- * Per row: action (int64), old, adv (fp32), ref (fp32, needed where kl_coef > 0) and an
+/* Clipped policy loss with a KL term over logits as in fh_xent_* (rows, vocab, ld, dtype),
+ * up to 2^31 - 1025 rows and columns. Per row: action (int64), old, adv (fp32), ref (fp32, needed where kl_coef > 0) and an
  * optional weight (fp32; NULL = 1). With lp = z[a] - log sum exp z, rho = exp(lp - old):
  *   l = -min(rho adv, clip(rho, 1 - clip_low, 1 + clip_high) adv)
  *       + kl_coef (exp(ref - lp) - (ref - lp) - 1),

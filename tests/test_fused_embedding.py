@@ -265,6 +265,9 @@ def test_c_abi_refusals():
     h, p, odd = lib(), ctypes.c_void_p(64), ctypes.c_void_p(72)
     assert h.fh_embed_scratch_bytes(-1, 4) == -1 and h.fh_embed_scratch_bytes(0, 4) == 0
     assert h.fh_embed_scratch_bytes(100, 4) >= 16 * 100
+    assert h.fh_embed_scratch_bytes(2 ** 31 - 1, 4) == -1             # 32-bit positions, a block past the end
+    assert h.fh_embed_scratch_bytes(2 ** 31 - 1025, 4) >= 16 * (2 ** 31 - 1025)
+    assert h.fh_embed_bwd(None, 0, 2 ** 31 - 1024, 1, 1, p, p, 1.0, -1, p, p) == 1
     assert h.fh_embed_fwd(None, 2, 1, 1, 1, p, p, 1.0, p) == 1        # dtype
     assert h.fh_embed_fwd(None, 0, 1, 0, 1, p, p, 1.0, p) == 1        # empty table
     assert h.fh_embed_fwd(None, 0, 1, 1, 1, None, p, 1.0, p) == 1

@@ -312,5 +312,7 @@ def test_c_abi_refusals():
     assert h.fh_policy_bwd_bwd(None, 0, 1, 4, 4, p, p, p, p, None, p, p, None) == 1
     assert h.fh_policy_bwd(None, 0, 1, 4, 4, p, p, ctypes.c_void_p(72), p, p) == 1  # stats not aligned
     assert h.fh_policy_stats_floats(-1, 4) == -1 and h.fh_policy_scratch_floats(1, 0) == -1
+    assert fwd(rows=2 ** 31 - 1024) == 1 and fwd(vocab=2 ** 31 - 1024, ld=2 ** 31) == 1
+    assert h.fh_policy_stats_floats(2 ** 31 - 1, 1) == -1 and h.fh_policy_stats_floats(2 ** 31 - 1025, 1) > 2 ** 33
     assert h.fh_policy_scratch_floats(1, 100) == 0 and h.fh_policy_scratch_floats(1, 1 << 20) > 0
     assert h.fh_policy_bwd_bwd(None, 0, 1, 1 << 20, 1 << 20, p, p, p, p, p, p, p, None) == 1  # needs scratch
