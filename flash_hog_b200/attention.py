@@ -88,7 +88,7 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
     if query.is_cuda and not attn_impl.transformed():
         causal, window = attn_impl._mask_args(mask_type)
         result = _capi.torch_ops().attention(query, key, value, causal, window,
-                                             attn_impl._mask_kw(mask_type).get("sinks", 0), scale,
+                                             attn_impl._mask_kw(mask_type).get("sinks", 0), float(scale),
                                              attn_impl._is_f32(query, policy))
     else:
         result, _ = _DotProductAttention.apply(query, key, value, mask_type, float(scale), policy)

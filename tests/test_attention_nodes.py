@@ -156,6 +156,38 @@ def test_some_inputs_without_gradient_hooks_and_checkpoint():
 
 
 @pytest.mark.gpu
+def test_one_tensor_as_all_three():
+    x = _qkv(torch.float32, hk=4)[0]
+    got = torch.autograd.grad(_call(x, x, x, is_causal=True).square().sum(), x)[0]
+    parts = [x.detach().clone().requires_grad_() for _ in range(3)]
+    want = sum(torch.autograd.grad(_call(*parts, is_causal=True).square().sum(), parts))
+    # Three fp32 terms added in another order: 2 * 2^-24 of the largest each.
+    assert (got - want).abs().max() <= 2.0 ** -22 * want.abs().max()
+
+
+@pytest.mark.gpu
+def test_inference_mode():
+    from flash_hog_b200 import fused
+
+    q, k, v = _qkv()
+    w = torch.randn(50, 16, device="cuda", requires_grad=True)
+    t = torch.arange(7, device="cuda")
+    z = torch.randn(7, 50, device="cuda", requires_grad=True)
+    zero, seed = torch.zeros(7, device="cuda"), torch.tensor([5], device="cuda")
+    calls = [lambda: _call(q, k, v, is_causal=True), lambda: fused.embedding(t, w, 2.0),
+             lambda: fused.dropout(q, 0.5, seed, residual=q), lambda: fused.policy_loss(z, t, zero, zero + 1)[0]]
+    for call in calls:
+        want = call()
+        assert want.requires_grad
+        with torch.inference_mode():
+            got = call()
+        assert got.is_inference() and not got.requires_grad and torch.equal(got, want)
+        with torch.no_grad():
+            got = call()
+        assert not got.requires_grad and torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_a_changed_input_is_noticed_and_graphs_are_freed():
     q, k, v = _qkv()
     out = _call(q, k, v)
