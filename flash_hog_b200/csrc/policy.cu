@@ -37,7 +37,6 @@ namespace fh {
 namespace {
 
 constexpr int kPolThreads = 256;
-constexpr int kPolWarps = kPolThreads / 32;
 // Columns up to which a row is one warp's (eight rows a block) instead of a block's: the
 // threads of a block would have less than two 16-byte loads each (100000 rows of 1000 bf16:
 // the sums take 299 us a block each, 61 us a warp each).
@@ -464,9 +463,14 @@ __global__ void __launch_bounds__(kPolThreads) policy_dots_kernel(PolicyArgs a, 
 }
 
 // The dot product <p, u> of the row comes from `part` (policy_dots_kernel) or, for whole rows,
-// is formed here: the second reading of z and u then comes from L2.
+// is formed here: the second reading of z and u then comes from L2, as far as the rows in
+// flight fit there. So four blocks an SM, and the second reading and gz, which this
+// kernel does not read again, marked as first to be evicted (4096 x 32000 bf16, all rows: 158 us; 206 with six
+// blocks, 169 with three, 120 at the copy rate). Holding the row in a cluster's shared memory
+// took 178 us: loading, joining and writing a row in turn leaves the memory idle, and clusters
+// that stay and load the next row meanwhile took 250 us or more.
 template <typename T, int NT>
-__global__ void __launch_bounds__(kPolThreads)
+__global__ void __launch_bounds__(kPolThreads, NT == 32 ? 6 : 4)
     policy_bwd_bwd_kernel(PolicyArgs a, int splits, const float* __restrict__ part, const float* __restrict__ g,
                           const T* __restrict__ u, T* __restrict__ gz, float* __restrict__ gg) {
   const Work<NT> wk(a.rows, splits);
@@ -505,7 +509,7 @@ __global__ void __launch_bounds__(kPolThreads)
   constexpr int kUnroll = NT == 32 ? 1 : 2;
 #pragma unroll kUnroll
   for (int i = wk.t; i < sp.nvec; i += NT) {
-    const uint4 rz = z4[i], ru = u4[i];
+    const uint4 rz = __ldcs(z4 + i), ru = __ldcs(u4 + i);
     float v[Span::E], x[Span::E];
     load_vec<T, Span::E>(reinterpret_cast<const T*>(&rz), v);
     load_vec<T, Span::E>(reinterpret_cast<const T*>(&ru), x);
@@ -519,7 +523,7 @@ __global__ void __launch_bounds__(kPolThreads)
     add_at(v, here, sp.vec(i), ks);
     uint4 o;
     store_vec<T, Span::E>(reinterpret_cast<T*>(&o), v);
-    out4[i] = o;
+    __stcs(out4 + i, o);
   }
   for (int i = wk.t; i < sp.scalars(cols.count); i += NT) {
     const int col = sp.scalar(i);

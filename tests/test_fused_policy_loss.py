@@ -57,6 +57,8 @@ def _statement(z, a, old, adv, ref, w, lo=0.2, hi=0.2, beta=0.0, norm=None):
 CASES = [  # rows, vocab, ld, offset
     (1, 1, 1, 0), (1, 2, 2, 0), (3, 7, 9, 1), (5, 1000, 1000, 0), (4, 1001, 1001, 0), (6, 1003, 1008, 3),
     (33, 4097, 4097, 0), (2, 131075, 131075, 0), (40, 16391, 16400, 1), (130, 8192, 8192, 0), (300, 513, 520, 0), (1, 40000, 40000, 5),
+    # Enough rows for a block each; rows of z and dz that reach 16 bytes at different columns.
+    (600, 2500, 2500, 0), (601, 8193, 8193, 0), (593, 16385, 16392, 8), (592, 32801, 32801, 3), (594, 9000, 9001, 0),
 ]
 
 
