@@ -295,30 +295,35 @@ __global__ void __launch_bounds__(kFinishThreads) policy_finish_kernel(PolicyArg
   const int r = blockIdx.x * kFinishThreads + threadIdx.x;
   double wl = 0.0, weight = 0.0;
   if (r < a.rows) {
+    // All that does not depend on another load first: the kernel's time is latency. (What
+    // `part` holds in a row of weight 0 is not used.)
     const float w = a.weights ? a.weights[r] : 1.f;
+    const float2* part = st.part + static_cast<size_t>(r) * splits;
+    const float2 part0 = part[0];
+    const long long act = a.actions[r];
+    const double adv = a.adv[r], old = a.old[r], ref = a.beta != 0.f ? a.ref[r] : 0.f;
     st.w[r] = w;
     if (w == 0.f) {
       a.lp[r] = 0.f;
       st.m[r] = st.rsum[r] = st.c[r] = st.dc[r] = 0.f;
     } else {
-      const float2* part = st.part + static_cast<size_t>(r) * splits;
-      float m = part[0].x;
+      const T* row = static_cast<const T*>(a.z) + static_cast<long long>(r) * a.ld;
+      const bool inside = act >= 0 && act < a.vocab;
+      const double za = inside ? to_f32(row[act]) : __int_as_float(0x7fc00000);
+      float m = part0.x;
       for (int k = 1; k < splits; ++k) m = fmaxf(m, part[k].x);
-      double sum = 0.0;
-      for (int k = 0; k < splits; ++k) {
+      double sum = splits == 1 ? part0.y : 0.0;
+      for (int k = 0; splits > 1 && k < splits; ++k) {
         const float2 p = part[k];
         sum += static_cast<double>(p.y) * (p.x == -INFINITY ? 1.f : exp_of(p.x, m));
       }
-      const T* row = static_cast<const T*>(a.z) + static_cast<long long>(r) * a.ld;
-      const long long act = a.actions[r];
-      double lp = __longlong_as_double(0x7ff8000000000000ll);
-      if (act >= 0 && act < a.vocab) lp = static_cast<double>(to_f32(row[act])) - static_cast<double>(m) - log(sum);
-      const double adv = a.adv[r], rho = exp(lp - static_cast<double>(a.old[r]));
+      const double lp = za - static_cast<double>(m) - log(sum);  // NaN for an action outside
+      const double rho = exp(lp - old);
       const double low = 1.0 - static_cast<double>(a.clip_low), high = 1.0 + static_cast<double>(a.clip_high);
       const bool open = !((adv > 0.0 && rho > high) || (adv < 0.0 && rho < low));
       double l = -adv * (open ? rho : adv > 0.0 ? high : low), dl = open ? -adv * rho : 0.0, ddl = dl;
       if (a.beta != 0.f) {
-        const double beta = a.beta, d = static_cast<double>(a.ref[r]) - lp, e = exp(d);
+        const double beta = a.beta, d = ref - lp, e = exp(d);
         l += beta * (e - d - 1.0);
         dl += beta * (1.0 - e);
         ddl += beta * e;
