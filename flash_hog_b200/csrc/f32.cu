@@ -360,9 +360,9 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas<HD>)
   float inv[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    inv[i] = l[i] > 0.f ? 1.f / l[i] : 0.f;
+    inv[i] = l[i] == 0.f ? 0.f : 1.f / l[i];  // no visible key: 0; NaN stays
     const int row = r0 + rg * 4 + i;
-    if (cg == 0 && row < s.Tq) lse[stat_index(s, b, h, row)] = l[i] > 0.f ? m[i] + logf(l[i]) : -INFINITY;
+    if (cg == 0 && row < s.Tq) lse[stat_index(s, b, h, row)] = l[i] == 0.f ? -INFINITY : m[i] + logf(l[i]);
   }
   store_rows<HD>(o, nullptr, s.sq, b, h, r0, s.Tq, acc, inv, rg, cg);
 }

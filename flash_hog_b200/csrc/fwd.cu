@@ -106,12 +106,10 @@ __device__ __forceinline__ float2 exp2_fma2(float2 x) {
   return r;
 }
 
-// The larger of two scores. NAN_OUT: NaN if either is (at the same cost), so that the row's
-// maximum, and with it every column of the row, becomes NaN: exp2_fma2 makes a large finite
-// number of one NaN column.
-template <bool NAN_OUT>
+// The larger of two scores, NaN if either is (at the cost of fmaxf), so that the row's
+// maximum, and with it every column of the row, becomes NaN: exp2_fma2 alone would make a
+// large finite number of a NaN column.
 __device__ __forceinline__ float score_max(float a, float b) {
-  if constexpr (!NAN_OUT) return fmaxf(a, b);
   float m;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
   return m;
@@ -364,17 +362,17 @@ __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
 #pragma unroll
       for (int c = 0; c < 8; ++c) mx[c] = __uint_as_float(v[c]);
 #pragma unroll
-      for (int i = 8; i < BN; ++i) mx[i & 7] = score_max<SNK>(mx[i & 7], __uint_as_float(v[i]));
+      for (int i = 8; i < BN; ++i) mx[i & 7] = score_max(mx[i & 7], __uint_as_float(v[i]));
 #pragma unroll
       for (int c = 4; c > 0; c >>= 1)
 #pragma unroll
-        for (int k = 0; k < c; ++k) mx[k] = score_max<SNK>(mx[k], mx[k + c]);
+        for (int k = 0; k < c; ++k) mx[k] = score_max(mx[k], mx[k + c]);
       const float tmax = mx[0] * sc2;  // log2 domain
-      const float m_new = score_max<SNK>(m_used, tmax);
+      const float m_new = score_max(m_used, tmax);
       float f = 1.f;  // rescale factor of O and l, applied before this tile's P is added
       if (j == 0) {
         m_used = m_new;
-      } else if (SNK ? !(m_new <= m_used + kRescaleLog2) : m_new > m_used + kRescaleLog2) {  // NaN: also
+      } else if (!(m_new <= m_used + kRescaleLog2)) {  // NaN: also
         f = ex2(m_used - m_new);
         m_used = m_new;
       }
@@ -396,7 +394,8 @@ __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
       // together when any of its rows needs it (the others multiply by f = 1).
       const bool warp_rescale = __any_sync(0xffffffffu, f != 1.f);
       if (!G::SEP_P && warp_rescale) rescale_o();
-      const float base = (m_used == -INFINITY) ? 0.f : m_used;
+      // A score of +inf makes its row NaN (inf - inf), in every column: inf * 0 + inf.
+      const float base = (m_used == -INFINITY) ? 0.f : fmaf(m_used, 0.f, m_used);
       uint32_t pk[BN / 2];
       // Column pairs through the packed fp32x2 instructions; the row sum in two
       // (even, odd) pair accumulators.
@@ -431,7 +430,7 @@ __global__ void __launch_bounds__(FPass<HD>::THREADS, FPass<HD>::CTAS)
     if (ok && nj > 0) ok = mbar_wait_warp(&bar_o_done[t], 0, &abort_flag);
     if (ok && nj > 0) {
       tc_fence_after();
-      const float inv = (l > 0.f) ? 1.f / l : 0.f;
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // no visible key: 0; NaN stays
       __nv_bfloat16* dst = a.o + q_row(sh, sr, row_ok ? row : 0, h);
 #pragma unroll
       for (int c = 0; c < HD; c += 16) {
