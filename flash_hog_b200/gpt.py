@@ -172,16 +172,39 @@ def penalty_objective(model: GPT, tokens: torch.Tensor, lam: float):
     return loss + lam * penalty, loss.detach(), penalty.detach()
 
 
+def _weight_share(weights, rows: int, device) -> torch.Tensor:
+    """ranks / (the sum of the policy weights over all ranks), fp32 on ``device``; 0 where that
+    sum is 0. One all-reduce of a scalar, no host synchronisation."""
+    import torch.distributed as dist
+
+    if weights is None:
+        total = torch.full((), float(rows), dtype=torch.float64, device=device)
+    else:
+        total = weights.sum(dtype=torch.float64)
+    dist.all_reduce(total)
+    return torch.where(total == 0, 0.0, dist.get_world_size() / total).float()
+
+
 def policy_objective(model: GPT, tokens: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor,
-                     lam: float = 0.0, **kwargs):
+                     lam: float = 0.0, distributed: bool = False, **kwargs):
     """(L + lam ||dL/dtheta||^2, L, log probabilities) for the clipped policy loss L of the
     tokens' own successors: ``tokens`` (B, T+1), everything else (B, T) over the T
     predictions (``weights`` of 0 for prompt and padding). ``kwargs`` are those of
-    ``fused.policy_loss``. With ``lam`` 0 no gradient is taken here."""
+    ``fused.policy_loss``. With ``lam`` 0 no gradient is taken here.
+
+    ``distributed``: L is normalised by the mean over the ranks of their sums of weights
+    (unless ``normalizer`` is given), so that the ranks' average of L, and of its gradient,
+    is the weighted mean over all ranks' rows, also where one has few of them or none."""
     b, t = tokens.shape[0], tokens.shape[1] - 1
     rows = {n: v.reshape(b * t) if isinstance(v, torch.Tensor) else v for n, v in kwargs.items()}
+    share = None
+    if distributed and rows.get("normalizer") is None:
+        share = _weight_share(rows.get("weights"), b * t, tokens.device)
+        rows["normalizer"] = 1.0
     loss, logprobs = fused_ops.policy_loss(model(tokens[:, :-1]).flatten(0, 1), tokens[:, 1:].reshape(b * t),
                                            old_logprobs.reshape(b * t), advantages.reshape(b * t), **rows)
+    if share is not None:
+        loss = loss * share
     total = loss
     if lam:
         grads = torch.autograd.grad(loss, [p for p in model.parameters() if p.requires_grad], create_graph=True)
@@ -290,10 +313,12 @@ class PenaltyStepGraph:
 def policy_step(model: GPT, tokens: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor,
                 lam: float = 0.0, optimizer=None, distributed: bool = False, autocast: bool = True, **kwargs):
     """One step on ``policy_objective``: its gradient, the data-parallel gradient average and
-    the optimizer update. Returns (loss, log probabilities of the tokens (B, T))."""
+    the optimizer update. Returns (loss, log probabilities of the tokens (B, T)); with
+    ``distributed`` the loss is this rank's share, whose average over the ranks is the loss.
+    A ``normalizer`` given with ``distributed`` divides each rank's own sum."""
     with torch.autocast(device_type=tokens.device.type, dtype=torch.bfloat16,
                         enabled=autocast and tokens.device.type == "cuda"):
-        total, loss, logprobs = policy_objective(model, tokens, old_logprobs, advantages, lam, **kwargs)
+        total, loss, logprobs = policy_objective(model, tokens, old_logprobs, advantages, lam, distributed, **kwargs)
     if optimizer is not None:
         optimizer.zero_grad(set_to_none=True)
     total.backward()
