@@ -144,8 +144,11 @@ int validate(const fh_attn_dims* d, SinkShape* out, float scale, int causal, boo
   out->br = causal == 2 ? 1 : 0;
   if (d->sinks < 0) return fail(kInvalidArgument, "sinks must be >= 0");
   if (d->sinks > 0 && !d->window) return fail(kInvalidArgument, "sinks need a sliding window");
-  out->window = d->window;
-  out->sinks = d->sinks;
+  // Past both lengths a window hides nothing and sinks are all keys: kept there, the kernels'
+  // sums of a row, a diagonal and a window stay in 32 bits.
+  const int longest = d->seq_q > d->seq_k ? d->seq_q : d->seq_k;
+  out->window = d->window < longest ? d->window : longest;
+  out->sinks = d->sinks < longest ? d->sinks : longest;
   out->total_q = d->seq_q;
   out->total_k = d->seq_k;
   if (varlen) {
@@ -161,7 +164,7 @@ int validate(const fh_attn_dims* d, SinkShape* out, float scale, int causal, boo
     out->diag = causal == 2 ? d->seq_k - d->seq_q : 0;
     // A window that hides nothing is the mask without sinks, but for the few rows that have
     // a kernel of their own with them.
-    if (d->seq_q + out->diag <= d->window && static_cast<long long>(d->seq_q) * out->G > kFewRows) out->sinks = 0;
+    if (d->seq_q + out->diag <= out->window && static_cast<long long>(d->seq_q) * out->G > kFewRows) out->sinks = 0;
   }
   out->sink_part = static_cast<float*>(d->sink_scratch);
   out->splits = 1;
