@@ -588,8 +588,11 @@ void bind(const py::dict& addresses) {
 
 PYBIND11_MODULE(_torch_ops, m) {
   m.def("bind", &bind);
-  m.def("attention", &attention);
-  m.def("embedding", &embedding);
-  m.def("dropout", &dropout);
-  m.def("policy_loss", &policy_loss);
+  // Without the interpreter's lock, as ctypes calls the library: a launch waits where the GPU's
+  // queue is full, and the allocator where it has to free memory.
+  using Unlocked = py::call_guard<py::gil_scoped_release>;
+  m.def("attention", &attention, Unlocked());
+  m.def("embedding", &embedding, Unlocked());
+  m.def("dropout", &dropout, Unlocked());
+  m.def("policy_loss", &policy_loss, Unlocked());
 }
