@@ -5,11 +5,14 @@
 the source tree, and so is ``_torch_ops.so``, the autograd nodes of dense
 attention and of ``fused``'s embedding, dropout and policy loss over that ABI
 (``csrc/torch_ops.cpp``). Object files are cached under ``_build/`` keyed by source and
-header modification times, so an unchanged tree rebuilds in well under a second.
+header modification times, so an unchanged tree rebuilds in seconds; the nodes are also
+built again beside another torch or Python than theirs.
 """
 
 from __future__ import annotations
 
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -71,17 +74,30 @@ def _link(objs, out):
         raise RuntimeError(f"link of {os.path.basename(out)} failed:\n{res.stdout}\n{res.stderr}")
 
 
+def _torch_ops_origin() -> str:
+    """What the nodes' library is built for: it loads beside this torch and Python alone."""
+    return "\n".join([sys.version, importlib.metadata.version("torch"), importlib.util.find_spec("torch").origin])
+
+
 def build_torch_ops() -> None:
-    """Compile ``csrc/torch_ops.cpp`` against torch's headers (host code only)."""
+    """Compile ``csrc/torch_ops.cpp`` against torch's headers (host code only), where the
+    library is older than its sources or was built for another torch or Python."""
     header = os.path.join(ROOT, "include", "flash_hog_b200.h")
-    if os.path.exists(TORCH_OPS_LIB) and os.path.getmtime(TORCH_OPS_LIB) >= max(
-            os.path.getmtime(TORCH_OPS_SOURCE), os.path.getmtime(header)):
-        return
+    stamp, origin = os.path.join(BUILD_DIR, "torch_ops.origin"), _torch_ops_origin()
+    if os.path.exists(TORCH_OPS_LIB) and os.path.exists(stamp):
+        with open(stamp) as f:
+            same = f.read() == origin
+        if same and os.path.getmtime(TORCH_OPS_LIB) >= max(os.path.getmtime(TORCH_OPS_SOURCE),
+                                                           os.path.getmtime(header)):
+            return
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
+    os.makedirs(BUILD_DIR, exist_ok=True)
+    if os.path.exists(stamp):  # until the build has ended
+        os.remove(stamp)
     includes = cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"], os.path.dirname(header)]
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_API_INCLUDE_EXTENSION_H",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *["-isystem" + i for i in includes],
@@ -90,6 +106,8 @@ def build_torch_ops() -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on torch_ops.cpp:\n{res.stdout}\n{res.stderr}")
+    with open(stamp, "w") as f:
+        f.write(origin)
 
 
 def build(verbose: bool = False) -> None:
