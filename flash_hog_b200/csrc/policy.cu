@@ -20,8 +20,9 @@
 // Every pass reads the logits once (the backward's backward twice, the second time from
 // L2) and is bound by memory. The exponentials are ex2((z - m) log2e) with the row maximum
 // m; the forward keeps m and 1 / sum, so the passes after it form the same p. The per-row
-// scalars (lp, rho, c, c') are formed in 64 bits: a ratio next to a clip border falls on
-// the side that it has.
+// scalars (lp, rho, c, c') are formed in 64 bits from that sum, whose exponentials and
+// additions are fp32: lp is off by some 1e-6 (1.6e-5 is the bound that the tests derive), and a
+// ratio that close to a clip border may fall on its other side.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -152,7 +153,7 @@ __device__ __forceinline__ uintptr_t addr(const void* p) { return reinterpret_ca
 // exp(z - m). The difference first: z and m may both be the type's lowest value.
 __device__ __forceinline__ float exp_of(float z, float m) { return pol_ex2((z - m) * kPLog2e); }
 
-// N / 2 pairs exp(z - m) of neighbouring columns, the arithmetic on fp32x2.
+// exp(z - m) of two neighbouring columns, the arithmetic on fp32x2.
 __device__ __forceinline__ float2 exp_of2(float a, float b, float2 neg_m) {
   const float2 x = __fmul2_rn(__fadd2_rn(make_float2(a, b), neg_m), make_float2(kPLog2e, kPLog2e));
   return make_float2(pol_ex2(x.x), pol_ex2(x.y));

@@ -237,6 +237,11 @@ def policy_loss(logits, actions, old_logprobs, advantages, *, ref_logprobs=None,
     ``weights`` (default: all 1) may be a boolean mask. Every input but the logits is a
     constant. ``logprobs`` (fp32, detached) are the lp, 0 in rows of weight 0.
     An action outside [0, vocab) in a weighted row gives NaN.
+
+    The per-row inputs, the clip bounds and ``kl_coef`` are taken in fp32, 64-bit ones
+    rounded to it. The exponentials and their sum are fp32: a log probability is accurate
+    to about 1e-5, and a ratio closer than that to a clip border may be counted on either
+    side of it.
     """
     return _capi.torch_ops().policy_loss(logits, actions, old_logprobs, advantages, ref_logprobs, weights, clip_low,
                                          clip_high, kl_coef, normalizer)

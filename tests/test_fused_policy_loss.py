@@ -318,3 +318,33 @@ def test_c_abi_refusals():
     assert h.fh_policy_stats_floats(2 ** 31 - 1, 1) == -1 and h.fh_policy_stats_floats(2 ** 31 - 1025, 1) > 2 ** 33
     assert h.fh_policy_scratch_floats(1, 100) == 0 and h.fh_policy_scratch_floats(1, 1 << 20) > 0
     assert h.fh_policy_bwd_bwd(None, 0, 1, 1 << 20, 1 << 20, p, p, p, p, p, p, p, None) == 1  # needs scratch
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [10, 1000, 32000, 131075])
+def test_the_side_of_a_clip_border(vocab, dtype):
+    """Ratios close to the borders fall on the side that they have, down to the bound on the log
+    probability (2 * REL and its rounding), and the others' rows carry their whole gradient."""
+    from flash_hog_b200 import fused
+
+    steps = [s * d for d in (2e-5, 4e-5, 1e-4, 1e-3) for s in (-1, 1)]
+    rows = 4 * len(steps)
+    g = torch.Generator().manual_seed(vocab)
+    z = (torch.randn(rows, vocab, generator=g) * 2.5).to(dtype).cuda()
+    a = torch.randint(0, vocab, (rows,), generator=g).cuda()
+    lp = torch.log_softmax(z.double(), 1).gather(1, a[:, None])[:, 0]
+    lo, hi = 0.2, 0.25
+    low, high = (1 + s * torch.tensor(c, dtype=torch.float32).double().item() for s, c in ((-1, lo), (1, hi)))
+    border = torch.tensor([math.log(high), math.log(low)] * 2, dtype=torch.float64).repeat_interleave(len(steps)).cuda()
+    adv = torch.tensor([1.0, 1.0, -1.0, -1.0]).repeat_interleave(len(steps)).cuda()
+    old = (lp - border - torch.tensor(steps * 4, dtype=torch.float64, device="cuda")).float()
+    distance = lp - old.double() - border  # after the rounding of old
+    assert (distance.abs() > 2 * REL + 2.0 ** -23 * lp.abs()).all()
+    rho = torch.exp(lp - old.double())
+    clipped = ((adv > 0) & (rho > high)) | ((adv < 0) & (rho < low))
+    assert 0 < clipped.sum() < rows
+    z.requires_grad_(True)
+    loss, _ = fused.policy_loss(z, a, old, adv, clip_low=lo, clip_high=hi)
+    (dz,) = torch.autograd.grad(loss, z)
+    assert torch.equal((dz == 0).all(1), clipped)
