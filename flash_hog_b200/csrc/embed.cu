@@ -469,7 +469,9 @@ int launch_embed_grad(bool bf16, int n, int vocab, int dim, const long long* tok
                         (kSortWarps + 1) * (1 << kMaxDigitBits) * 4) != kOk)
     return kLaunchFailed;
   // CTAs that fill: two per SM, or fewer when there is little to fill. (With one per SM
-  // the clusters of a GPC share its SMs unevenly: 98 MB took 26 us.)
+  // the clusters of a GPC share its SMs unevenly: 98 MB took 26 us.) At digits of 10 bits
+  // (tables of 512 to 1023 rows and of 2^18 to 2^20, say) the launch's shared memory, 135 KB
+  // for the filling CTAs too, leaves room for one on an SM: they run one after the other.
   const long long want = (so.fill_vecs + 8ll * kSortThreads - 1) / (8ll * kSortThreads) + 1;
   const long long most = 2 * sm_count() - kSortCluster;
   const long long ctas = want < most ? want : most;

@@ -275,3 +275,33 @@ def test_c_abi_refusals():
     assert h.fh_embed_bwd(None, 0, 1, 1, 1, p, p, 1.0, -1, odd, p) == 1  # dw not aligned
     assert h.fh_embed_bwd(None, 0, 1, 1, 1, p, p, 1.0, -1, p, None) == 1
     assert h.fh_embed_bwd_bwd(None, 0, -1, 1, 1, p, p, 1.0, -1, p) == 1
+
+
+# Lists long enough for the chunks of 64 (from 151584 tokens on) and of 128 (303168).
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [160000, 163841, 320000, 327681])
+@pytest.mark.parametrize("vocab,skew", [(300000, 0), (5000, 8), (1, 0)])
+def test_long_lists(vocab, skew, n, dtype):
+    from flash_hog_b200 import fused
+
+    w, t, dy = _inputs(n, vocab, 8, dtype, n + vocab, skew)
+    w.requires_grad_(True)
+    (dw,) = torch.autograd.grad(fused.embedding(t, w, 0.5), w, dy)
+    _check_grad(dw, t, dy, vocab, 0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [160000, 320000])
+@pytest.mark.parametrize("run", [63, 64, 65, 127, 128, 129, 191, 256, 1151])
+def test_runs_around_the_borders_of_long_chunks(run, n):
+    """Runs that end at, one before and one after multiples of 64 and 128, up to those that a
+    block joins together."""
+    from flash_hog_b200 import fused
+
+    vocab = (n + run - 1) // run
+    w, _, dy = _inputs(n, vocab, 4, torch.float32, run)
+    t = (torch.arange(n) // run)[torch.randperm(n, generator=torch.Generator().manual_seed(run))].cuda()
+    w.requires_grad_(True)
+    (dw,) = torch.autograd.grad(fused.embedding(t, w), w, dy)
+    _check_grad(dw, t, dy, vocab, 1.0)
