@@ -108,7 +108,11 @@ class GPT(nn.Module):
     With ``cfg.dropout`` each forward in training mode takes the next seed of the buffer
     ``dropout_seed`` (an int64 tensor of one element, from 0; give data-parallel ranks
     different starts): the masks of a step are a function of it, and steps replayed as a
-    CUDA graph advance it too."""
+    CUDA graph advance it too. It is not part of the state dict: save and restore it with a
+    checkpoint, or a resumed run draws its first masks again.
+
+    On the fused kernels a token outside the vocabulary does not stop the program, as
+    ``nn.Embedding``'s check on the device does: its row is NaN, and with it the loss."""
 
     def __init__(self, cfg: GPTConfig, attention: str = "flash", fused: bool | None = None):
         super().__init__()
@@ -141,6 +145,8 @@ class GPT(nn.Module):
 
     def forward(self, tokens):
         t = tokens.shape[1]
+        if t > self.cfg.seq_len:  # the fused lookup would give rows of NaN
+            raise IndexError(f"{t} tokens a row, but the model has {self.cfg.seq_len} positions")
         x = self.wte(tokens)
         if not self.fused and self.cfg.embed_scale != 1.0:
             x = x * self.cfg.embed_scale

@@ -200,3 +200,10 @@ def test_policy_steps_under_autocast_run():
                                 ref_logprobs=lp, kl_coef=0.1)
         assert loss.isfinite() and new.isfinite().all()
     assert all(p.isfinite().all() for p in model.parameters())
+
+
+@pytest.mark.parametrize("attention", ["naive", "flash"])
+def test_more_tokens_than_positions_are_refused(attention):
+    model = GPT(GPTConfig(n_layer=1, d_model=64, n_head=1, d_mlp=64, vocab=50, seq_len=16), attention=attention)
+    with pytest.raises(IndexError):
+        model(torch.zeros(1, 17, dtype=torch.long))
