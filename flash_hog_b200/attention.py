@@ -24,7 +24,7 @@ backward's query pass at dO = 0) and the backward's jvp (double backward plus
 first-order backward, ``fh_attn_jvp_bwd``) on the kernels.
 
 Plain calls -- no transform or forward mode at work -- of dense attention take the same
-three rules as C++ nodes (``csrc/torch_ops.cpp``), which cost a third of the host time.
+three rules as C++ nodes (``csrc/torch_ops.cpp``), which cost half of the host time.
 
 Both Functions, and ``flash_bwdbwd``, also have batching rules for
 ``torch.func.vmap``: the vmapped axis is folded into the batch axis and the
@@ -72,7 +72,10 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
     ``sliding_window_length`` W (each query sees the W keys ending at its diagonal) and,
     with a window, ``sink_tokens`` S (the first S keys stay visible behind it: query i
     sees key j iff j <= diag_i and (j > diag_i - W or j < S)).
-    A query that sees no key gets a zero output.
+    A query that sees no key gets a zero output. A NaN or a score of +inf among the visible
+    keys makes the query's row NaN. A hidden key's score does not count, but its key and
+    value must be finite where it shares a tile (up to 128 keys) with visible ones: the
+    products go over whole tiles.
     """
     if scale is None:
         scale = query.shape[-1] ** -0.5
@@ -115,6 +118,7 @@ def dot_product_attention_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, 
     sinks, up to rounding for sequences of so few queries that the dense call runs its
     kernel for single tokens). Computes with bf16 operands (any input dtype; results in the
     input dtype).
+    A NaN or infinity in one sequence may reach the next to it, whose rows share its tiles.
     """
     if query.ndim != 3 or key.ndim != 3 or value.ndim != 3:
         raise ValueError("packed tensors are (total, heads, head_dim)")
@@ -122,8 +126,8 @@ def dot_product_attention_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, 
         scale = query.shape[-1] ** -0.5
     mask = _mask_of(is_causal, causal_alignment, sliding_window_length, sink_tokens)
     packed = PackedSequences(mask, cu_seqlens_q, cu_seqlens_k, int(max_seqlen_q), int(max_seqlen_k))
-    result, _ = _function(_Plain).apply(query.unsqueeze(0), key.unsqueeze(0), value.unsqueeze(0),
-                                                           packed, float(scale), "bf16")
+    result, _ = _function(_Plain).apply(query.unsqueeze(0), key.unsqueeze(0), value.unsqueeze(0), packed,
+                                        float(scale), "bf16")
     return result.squeeze(0)
 
 
@@ -195,8 +199,8 @@ class _DotProductAttention(torch.autograd.Function):
                 mask_type=ctx.mask_type, scale=ctx.scale, res=(query, key, value, activation, out), g=g,
                 policy=ctx.policy)
         else:
-            dq, dk, dv = _function(_PlainBwd).apply(query, key, value, activation, out, g,
-                                                                          ctx.mask_type, ctx.scale, ctx.policy)
+            dq, dk, dv = _function(_PlainBwd).apply(query, key, value, activation, out, g, ctx.mask_type, ctx.scale,
+                                                    ctx.policy)
         return dq, dk, dv, None, None, None
 
     @staticmethod

@@ -133,5 +133,5 @@ class _FlashBwdBwd(torch.autograd.Function):
         return (_unfold(dq2, size), _unfold(dk2, size), _unfold(dv2, size), _unfold(ddo, size), stats), (0, 0, 0, 0, 1)
 
 
-# As for the Functions of attention.py: the signature is worked out once.
+# torch binds the arguments by the signature in every call: worked out once.
 _FlashBwdBwd.forward.__signature__ = inspect.signature(_FlashBwdBwd.forward)

@@ -210,7 +210,7 @@ __host__ __device__ __forceinline__ int sink_tiles(const SinkShape& s) {
 // Parts into which the key passes cut the queries of a key tile that holds a sink: every
 // query sees it, where an ordinary tile is seen by about window + kBM of them, so a CTA
 // with a whole one may still run when the others are done (causal B1 H8 Hk2 S8000 D128,
-// window 2048: dK/dV 476 us whole, 128 us in 4 parts and the join 3 us). As many parts as
+// window 2048, 4 sinks: dK/dV 512 us whole, 136 us in 4 parts and the join 3 us). As many parts as
 // make them about equal to ordinary tiles, but no more than it takes to fill the GPU a few
 // times over: each costs a partial sum of 2 x kBM x head_dim floats and a share of the join.
 inline int sink_splits(const SinkShape& s) {

@@ -19,6 +19,10 @@
 // core's math rate; the key-tiled pass folds -L/scale and -D into its score
 // accumulators with one bias MMA per tile, so its elementwise warps read no
 // per-query statistics.
+//
+// P and dS enter the products after them as bf16, the operand type of those products;
+// sums and statistics are fp32. At B4 H16 S2048 D64, window 512, the gradients' error is
+// 0.0025 of their size (root mean square); rounding them to bf16 at the end alone is 0.0017.
 
 #include <cuda_runtime.h>
 

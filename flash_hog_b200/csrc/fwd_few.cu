@@ -306,6 +306,8 @@ int launch_few(const FewArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
+// With sinks only: a token under a plain window would have the same list of keys and the same
+// gain, but keeps the tile kernel, whose results such calls have always had bit for bit.
 bool fwd_few_applies(const SinkShape& s) {
   return s.sinks > 0 && static_cast<long long>(s.Tq) * s.G <= kFewRows && s.Hk <= 65535 && s.B <= 65535;
 }

@@ -1,6 +1,7 @@
 """NaN and infinities in what attention reads: a visible NaN, or a score of +inf, makes the
-rows that see it NaN (output and log-sum-exp), a score of -inf counts as 0, and what a mask
-hides does not count -- with every mask, whichever kernel it takes and wherever the key lies."""
+rows that see it NaN (output and log-sum-exp), a score of -inf counts as 0, and a hidden
+key's score does not count -- with every mask, whichever kernel it takes and wherever the key
+lies."""
 
 import pytest
 import torch
