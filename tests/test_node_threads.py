@@ -50,6 +50,7 @@ def test_other_threads_run_while_a_launch_waits(name):
         done.set()
         thread.join()
     gap = max(b - a for a, b in zip(ticks, ticks[1:]))
-    # The launches that find the queue full wait for most of the second; a thread that only
-    # shares the interpreter gets it every few milliseconds.
-    assert took > 0.5 and gap < 0.25 * took
+    # The first launch that finds the queue full (after a thousand or so, some 20 ms) waits for
+    # the rest of the second; a thread that only shares the interpreter gets it every few
+    # milliseconds.
+    assert took > 0.5 and gap < 0.5 * took
